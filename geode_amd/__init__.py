@@ -55,6 +55,40 @@ class GvStateInfo(_c.Structure):
                 ("has_hidden", _c.c_int32)]
 
 
+class GvPagedKv(_c.Structure):
+    _fields_ = [(n, _c.c_int32) for n in ("type", "n_kv_heads", "head_dim", "page_size", "n_pages")] + \
+               [(n, _P) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, _c.c_int64) for n in ("page_stride", "head_stride", "pos_stride")]
+
+
+class GvPagedBatch(_c.Structure):
+    _fields_ = [(n, _c.c_int32) for n in ("n_seqs", "n_rows", "max_rows", "max_len")] + \
+               [(n, _P) for n in ("row_start", "lens", "pages")] + [("ld_pages", _c.c_int64)]
+
+
+class GvAppendRows(_c.Structure):
+    _fields_ = [("type", _c.c_int32), ("n_heads", _c.c_int32), ("q", _P), ("k", _P), ("v", _P)] + \
+               [(n, _c.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
+               [("q_norm", _P), ("k_norm", _P), ("eps", _c.c_float), ("rope_dim", _c.c_int32),
+                ("interleaved", _c.c_int32), ("cos", _P), ("sin", _P), ("n_positions", _c.c_int32),
+                ("positions", _P), ("q_type", _c.c_int32), ("q_out", _P), ("q_out_row", _c.c_int64)]
+
+
+class GvAttentionRows(_c.Structure):
+    _fields_ = [("type", _c.c_int32), ("n_heads", _c.c_int32), ("q", _P), ("q_row", _c.c_int64), ("out", _P),
+                ("out_row", _c.c_int64), ("lse", _P), ("scale", _c.c_float), ("visible", _P)]
+
+
+class GvLogitsRules(_c.Structure):
+    _fields_ = [("repetition", _P), ("frequency", _P), ("presence", _P), ("tokens", _P), ("n_tokens", _c.c_int64),
+                ("begin", _P), ("generated", _P), ("end", _P), ("bias_token", _P), ("bias_value", _P),
+                ("n_biases", _c.c_int64), ("bias_begin", _P), ("bias_end", _P), ("masks", _P),
+                ("n_masks", _c.c_int32), ("ld_mask", _c.c_int64), ("mask_of", _P)]
+
+
+# element types of the paged cache's calls and gv_process_logits
+F32, F16, BF16, I8 = range(4)
+
 # tensor kinds of gv_model_adopt
 EMBED, LM_HEAD, FINAL_NORM, IN_NORM, POST_NORM, QKV, O, Q_NORM, K_NORM, ROUTER, SHARED_GATE, EXPERT, \
     SHARED_EXPERT, KV, KV_I8 = 0, 1, 2, 3, 4, 5, 8, 9, 10, 11, 12, 13, 14, 17, 18
@@ -138,6 +172,12 @@ SIGNATURES = {
     "gv_sampler_paths": (_c.c_int, [_P, _P]),
     "gv_accept_textbook": (_c.c_int, [_P, _P, _c.c_int64, _c.c_int, _c.c_int, _c.c_float, _c.c_float, _c.c_int,
                                       _P, _P, _c.c_float, _P]),
+    "gv_paged_append": (_c.c_int, [_c.POINTER(GvPagedKv), _c.POINTER(GvPagedBatch), _c.POINTER(GvAppendRows)]),
+    "gv_paged_attention_workspace_bytes": (_c.c_size_t, [_c.POINTER(GvPagedKv), _c.POINTER(GvPagedBatch), _c.c_int]),
+    "gv_paged_attention": (_c.c_int, [_c.POINTER(GvPagedKv), _c.POINTER(GvPagedBatch), _c.POINTER(GvAttentionRows),
+                                      _P, _c.c_size_t]),
+    "gv_process_logits": (_c.c_int, [_c.POINTER(GvLogitsRules), _P, _c.c_int, _c.c_int64, _c.c_int, _c.c_int, _P,
+                                     _c.c_int64]),
 }
 
 # kernel classes of a verify step (gv_model_time_kernel)
@@ -358,6 +398,144 @@ def sampler_paths():
     a, b = _c.c_int64(0), _c.c_int64(0)
     check(_lib().gv_sampler_paths(_c.byref(a), _c.byref(b)), "gv_sampler_paths")
     return a.value, b.value
+
+
+def _bits16(x, type_):
+    """float32 values as the bits of a 16-bit type (bf16: rounded to nearest even by hand; numpy has none)"""
+    x = np.ascontiguousarray(x, np.float32)
+    if type_ == F16:
+        return x.astype(np.float16).view(np.uint16)
+    b = x.view(np.uint32)
+    r = ((b + 0x7FFF + ((b >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(x), np.uint16(0x7FC0), r)
+
+
+def _from_bits(a, type_):
+    """an array of an element type's bits (float32, uint16 or int8) as float32 values"""
+    if type_ == F16:
+        return a.view(np.float16).astype(np.float32)
+    if type_ == BF16:
+        return (a.astype(np.uint32) << 16).view(np.float32)
+    return a.astype(np.float32)
+
+
+_NP_TYPE = {F32: np.float32, F16: np.uint16, BF16: np.uint16, I8: np.int8}
+
+
+def _typed(x, type_):
+    """a float array as a device buffer of a floating element type"""
+    return DeviceBuffer.from_array(np.ascontiguousarray(x, np.float32) if type_ == F32 else _bits16(x, type_))
+
+
+class PagedCache:
+    """One layer's paged key/value cache on the device ([page][head][position][dim], or [page][position][head][dim]
+    with by_position), as gv_paged_append writes it and gv_paged_attention reads it."""
+
+    def __init__(self, type_, n_pages, page_size, n_kv_heads, head_dim, by_position=False):
+        self.type, self.by_position = type_, by_position
+        self.shape = (n_pages, page_size, n_kv_heads, head_dim) if by_position else (n_pages, n_kv_heads, page_size, head_dim)
+        n = n_pages * page_size * n_kv_heads * head_dim * np.dtype(_NP_TYPE[type_]).itemsize
+        self.k, self.v = DeviceBuffer(n), DeviceBuffer(n)
+        self.scale_shape = (n_pages, n_kv_heads, page_size)
+        scale_bytes = int(np.prod(self.scale_shape)) * 4
+        self.k_scale, self.v_scale = (DeviceBuffer(scale_bytes), DeviceBuffer(scale_bytes)) if type_ == I8 else (None, None)
+        for b in (self.k, self.v, self.k_scale, self.v_scale):
+            if b is not None:
+                b.zero()
+        self.desc = GvPagedKv(type_, n_kv_heads, head_dim, page_size, n_pages, self.k.ptr, self.v.ptr,
+                              self.k_scale.ptr if self.k_scale else None, self.v_scale.ptr if self.v_scale else None,
+                              page_size * n_kv_heads * head_dim, head_dim if by_position else page_size * head_dim,
+                              n_kv_heads * head_dim if by_position else head_dim)
+
+    def read(self, which):
+        """the pool's keys ("k") or values ("v") as the float32 values they stand for, [page, head, position, dim]"""
+        a = _from_bits(getattr(self, which).download(_NP_TYPE[self.type], self.shape), self.type)
+        a = a.transpose(0, 2, 1, 3) if self.by_position else a
+        if self.type == I8:
+            a = a * getattr(self, which + "_scale").download(np.float32, self.scale_shape)[..., None]
+        return a
+
+    def write(self, which, values, scales=None):
+        """the pool's keys or values from floats [page, head, position, dim] (an int8 pool: codes and their scales)"""
+        a = np.ascontiguousarray(np.asarray(values).transpose(0, 2, 1, 3) if self.by_position else values)
+        getattr(self, which).upload(a.astype(np.int8) if self.type == I8 else _bits16(a, self.type))
+        if self.type == I8:
+            getattr(self, which + "_scale").upload(np.ascontiguousarray(scales, np.float32))
+
+
+class PagedBatch:
+    """The rows of one step over a paged cache: each sequence's rows, length (its new rows included) and pages."""
+
+    def __init__(self, rows, lens, pages, n_rows=None, max_rows=None, max_len=None, first_row=0):
+        rows, lens = np.asarray(rows, np.int32), np.asarray(lens, np.int32)
+        pages = np.ascontiguousarray(pages, np.int32)
+        start = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32) + np.int32(first_row)
+        self.bufs = [DeviceBuffer.from_array(a) for a in (start, lens, pages)]
+        self.desc = GvPagedBatch(rows.size, int(n_rows if n_rows is not None else start[-1]),
+                                 int(max_rows if max_rows is not None else max(1, rows.max())),
+                                 int(max_len if max_len is not None else lens.max()), *[b.ptr for b in self.bufs],
+                                 pages.shape[1])
+
+
+def paged_append(cache, batch, q, k, v, *, type_=F32, q_type=F32, q_norm=None, k_norm=None, eps=1e-6, rope_dim=0,
+                 interleaved=False, cos=None, sin=None, positions=None):
+    """New rows (float [n_rows, heads, head_dim] each, q None: none) normalized, rotated and appended to a PagedCache;
+    the queries as float32 values [n_rows, heads, head_dim]"""
+    T, hd = k.shape[0], cache.desc.head_dim
+    dq, dk, dv = (None if x is None else _typed(x, type_) for x in (q, k, v))
+    dev = {n: None if a is None else DeviceBuffer.from_array(np.ascontiguousarray(a, t))
+           for n, a, t in (("q_norm", q_norm, np.float32), ("k_norm", k_norm, np.float32), ("cos", cos, np.float32),
+                           ("sin", sin, np.float32), ("positions", positions, np.int32))}
+    nh = 0 if q is None else q.shape[1]
+    out = DeviceBuffer(T * nh * hd * np.dtype(_NP_TYPE[q_type]).itemsize)
+    out.zero()
+    r = GvAppendRows(type_, nh, dq.ptr if dq else None, dk.ptr, dv.ptr, nh * hd, hd, k.shape[1] * hd, hd,
+                     v.shape[1] * hd, hd, *[dev[n].ptr if dev[n] else None for n in ("q_norm", "k_norm")], eps, rope_dim,
+                     int(interleaved), *[dev[n].ptr if dev[n] else None for n in ("cos", "sin")],
+                     0 if cos is None else np.shape(cos)[0], dev["positions"].ptr if dev["positions"] else None, q_type,
+                     out.ptr, nh * hd)
+    check(_lib().gv_paged_append(_c.byref(cache.desc), _c.byref(batch.desc), _c.byref(r)), "gv_paged_append")
+    check(_lib().gv_synchronize(), "gv_paged_append")
+    return _from_bits(out.download(_NP_TYPE[q_type], (T, nh, hd)), q_type)
+
+
+def paged_attention(cache, batch, q, *, type_=F32, scale=None, visible=None):
+    """Attention of the rows' queries (float [n_rows, heads, head_dim]) over a PagedCache: (out, log-sum-exp) as
+    float32; visible: each row's bits of its sequence's rows (None: a chain). Rows of no sequence give zeros."""
+    T, nh, hd = q.shape
+    dq, out, lse = _typed(q, type_), DeviceBuffer(q.size * np.dtype(_NP_TYPE[type_]).itemsize), DeviceBuffer(T * nh * 4)
+    out.zero()
+    lse.zero()
+    dvis = None if visible is None else DeviceBuffer.from_array(np.ascontiguousarray(visible, np.uint32))
+    n = _lib().gv_paged_attention_workspace_bytes(_c.byref(cache.desc), _c.byref(batch.desc), nh)
+    ws = DeviceBuffer(n)
+    r = GvAttentionRows(type_, nh, dq.ptr, nh * hd, out.ptr, nh * hd, lse.ptr,
+                        hd ** -0.5 if scale is None else scale, dvis.ptr if dvis else None)
+    check(_lib().gv_paged_attention(_c.byref(cache.desc), _c.byref(batch.desc), _c.byref(r), ws.ptr, n),
+          "gv_paged_attention")
+    check(_lib().gv_synchronize(), "gv_paged_attention")
+    return _from_bits(out.download(_NP_TYPE[type_], (T, nh, hd)), type_), lse.download(np.float32, (T, nh))
+
+
+def process_logits(logits, *, type_=F32, tokens=None, begin=None, end=None, generated=None, repetition=None,
+                   frequency=None, presence=None, bias_token=None, bias_value=None, bias_begin=None, bias_end=None,
+                   masks=None, mask_of=None, in_place=False):
+    """gv_process_logits of rows of logits (float [rows, V]): the rows after the rules, float32 [rows, V]. The arrays are
+    those of gv_logits_rules; masks: uint32 [n_masks, words]."""
+    rows, V = logits.shape
+    src = _typed(logits, type_)
+    out = src if in_place else DeviceBuffer(rows * V * 4)
+    kinds = dict(repetition=np.float32, frequency=np.float32, presence=np.float32, tokens=np.int32, begin=np.int32,
+                 generated=np.int32, end=np.int32, bias_token=np.int32, bias_value=np.float32, bias_begin=np.int32,
+                 bias_end=np.int32, masks=np.uint32, mask_of=np.int32)
+    given = locals()
+    dev = {n: DeviceBuffer.from_array(np.ascontiguousarray(given[n], t)) for n, t in kinds.items() if given[n] is not None}
+    r = GvLogitsRules(**{n: b.ptr for n, b in dev.items()}, n_tokens=0 if tokens is None else len(tokens),
+                      n_biases=0 if bias_token is None else len(bias_token),
+                      n_masks=0 if masks is None else len(masks), ld_mask=0 if masks is None else np.shape(masks)[1])
+    check(_lib().gv_process_logits(_c.byref(r), src.ptr, type_, V, rows, V, out.ptr, V), "gv_process_logits")
+    check(_lib().gv_synchronize(), "gv_process_logits")
+    return out.download(np.float32, (rows, V))
 
 
 class Pack:

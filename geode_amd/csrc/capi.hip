@@ -10,6 +10,7 @@
 #include "../../include/geode_verify.h"
 #include "common.hpp"
 #include "kernels.hpp"
+#include "paged.hpp"
 
 namespace gv {
 
@@ -34,6 +35,7 @@ Runtime &rt() {
 }
 
 hipStream_t stream() { return rt().stream; }
+int device() { return rt().device; }
 
 // Every source file's copy of the operands' mode to `exact`, when it differs: the device idle before (no kernel may
 // read a copy while it changes) and after
@@ -181,7 +183,7 @@ int gv_memset(void *dst, int value, size_t bytes) {
 int gv_synchronize(void) {
     if (ensure_init() != 0) return -1;
     GV_CHECK_HIP(hipStreamSynchronize(stream()));
-    return 0;
+    return take_queued_faults();
 }
 
 int gv_event_record(void) {

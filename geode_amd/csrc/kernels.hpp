@@ -77,6 +77,7 @@ int64_t tiles_per_wg(int64_t ntiles, int waves, int ntt);
 
 // the library's stream and lazy device set-up (capi.hip)
 hipStream_t stream();
+int device();   // the GPU it runs on (-1 before gv_init)
 int ensure_init();
 
 // elementwise helpers (misc.hip)

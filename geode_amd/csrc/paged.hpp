@@ -1,0 +1,127 @@
+// paged.hpp - what the calls over several conversations share: the paged cache and the batch as the kernels take them,
+// the checks of the host's arguments, the device's own of what lies in device memory, and the faults it reports.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/geode_verify.h"
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace gv {
+
+// ---------------------------------------------------------------- faults met in device memory
+// A kernel that meets one sets its word in pinned host memory (a plain store: every writer writes 1); gv_synchronize
+// reads the words once the stream is idle, clears them and fails.
+enum QueuedFault { kFaultRows = 0, kFaultPage = 1, kFaultPosition = 2, kFaultRange = 3, kFaultCount = 4 };
+int *queued_faults();        // the words as the device addresses them (null: no memory, the error set)
+int take_queued_faults();    // 0, or -1 and a message, the words cleared (the stream idle)
+__device__ inline void queue_fault(int *words, int kind) {
+    *reinterpret_cast<volatile int *>(words + kind) = 1;
+}
+
+// The library's GPU current for the calling thread while a call runs, whatever the thread's own choice.
+struct OnDevice {
+    int before = -1;
+    bool ok = true;
+    OnDevice();
+    ~OnDevice();
+};
+
+struct KvView {
+    char *k, *v;
+    float *ks, *vs;
+    int64_t page_stride, head_stride, pos_stride;   // elements
+    int nkv, hd, page, n_pages;
+};
+struct BatchView {
+    const int *row_start, *lens, *pages;
+    int64_t ld_pages;
+    int n_seqs, n_rows, max_rows, max_len;
+};
+inline KvView kv_view(const gv_paged_kv &c) {
+    return KvView{static_cast<char *>(c.k), static_cast<char *>(c.v), c.k_scale, c.v_scale, c.page_stride, c.head_stride,
+                  c.pos_stride, c.n_kv_heads, c.head_dim, c.page_size, c.n_pages};
+}
+inline BatchView batch_view(const gv_paged_batch &b) {
+    return BatchView{b.row_start, b.lens, b.pages, b.ld_pages, b.n_seqs, b.n_rows, b.max_rows, b.max_len};
+}
+
+inline bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+inline int64_t type_bytes(int type) { return type == GV_F32 ? 4 : type == GV_I8 ? 1 : 2; }
+inline bool float_type(int type) { return type == GV_F32 || type == GV_F16 || type == GV_BF16; }
+
+// a refused argument: the call's name (a `call` in scope) before the reason
+#define GV_CHECK_ARG(cond, what) GV_REQUIRE(cond, std::string(call) + ": " + (what))
+// 0, or -1 and the reason
+int check_kv(const gv_paged_kv *c, const char *call);
+int check_batch(const gv_paged_batch *b, const gv_paged_kv *c, const char *call);
+
+#ifdef __HIPCC__
+// The sequence of row t: the first whose rows end behind t (n_seqs: none). A 64-way search by a whole wave, two loads
+// deep up to 4,096 sequences. Row starts that descend give some sequence of the batch, which its own check refuses.
+__device__ inline int seq_of_row(const BatchView &b, int t) {
+    const int lane = threadIdx.x & 63;
+    const int *end = b.row_start + 1;
+    int lo = 0, hi = b.n_seqs;
+    while (hi - lo > 64) {
+        const int step = (hi - lo + 63) / 64;
+        const int i = min(lo + (lane + 1) * step, hi) - 1;
+        const int full = __popcll(__ballot(end[i] <= t));
+        lo = min(lo + full * step, hi);
+        hi = min(lo + step, hi);
+    }
+    const int i = lo + lane;
+    const bool before = i < hi && end[min(i, b.n_seqs - 1)] <= t;
+    return lo + __popcll(__ballot(before));
+}
+
+// a sequence's rows and positions as the batch gives them, and whether they fit it
+struct Seq {
+    int first, rows, len;   // row_start, rows, positions in the cache
+    bool fits;
+};
+__device__ inline Seq seq_load(const BatchView &b, int i) {
+    const int a = b.row_start[i], e = b.row_start[i + 1], len = b.lens[i];
+    const int n = static_cast<int>(static_cast<unsigned>(e) - static_cast<unsigned>(a));   // (used where it fits)
+    return Seq{a, n, len, a >= 0 && e >= a && e <= b.n_rows && n <= b.max_rows && len >= n && len <= b.max_len};
+}
+
+// 32-bit floats to the 16-bit types, rounded to nearest even
+__device__ inline uint32_t pack_f16(float lo, float hi) {
+    return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, f16_of(lo))) |
+           static_cast<uint32_t>(__builtin_bit_cast(uint16_t, f16_of(hi))) << 16;
+}
+__device__ inline uint32_t pack_bf16(float lo, float hi) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ inline float half_lo(uint32_t w) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w))); }
+__device__ inline float half_hi(uint32_t w) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w >> 16))); }
+__device__ inline float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ inline float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xFFFF0000u); }
+
+// four consecutive values of a type as floats (16 or 8 bytes, aligned), and four floats stored as a type
+template <int TYPE>
+__device__ inline float4 load4(const char *p) {
+    if constexpr (TYPE == GV_F32) {
+        return *reinterpret_cast<const float4 *>(p);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2 *>(p);
+        if constexpr (TYPE == GV_F16) return float4{half_lo(w.x), half_hi(w.x), half_lo(w.y), half_hi(w.y)};
+        return float4{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
+    }
+}
+template <int TYPE>
+__device__ inline void store4(char *p, float4 x) {
+    if constexpr (TYPE == GV_F32) *reinterpret_cast<float4 *>(p) = x;
+    else if constexpr (TYPE == GV_F16) *reinterpret_cast<uint2 *>(p) = uint2{pack_f16(x.x, x.y), pack_f16(x.z, x.w)};
+    else *reinterpret_cast<uint2 *>(p) = uint2{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)};
+}
+#endif
+
+}  // namespace gv

@@ -1,0 +1,172 @@
+// paged_attn.hip - gv_paged_attention: its launches, its workspace, and the joining of a sequence's chunks.
+#include <algorithm>
+#include <string>
+
+#include "paged_attn.hpp"
+
+namespace gv {
+
+// A workgroup a (row, query head): the chunks' sums times exp(their maximum - the largest), over the sum of weights.
+// A group of lanes holds a chunk's dims (four a lane), the groups take chunks in turn and are added in LDS.
+// Bound by latency (the row's sequence, the maxima, the sums): the sums were just written and lie in the caches.
+constexpr int kJoinThreads = 256;
+struct JoinArgs {
+    BatchView b;
+    const float *parts, *ml;
+    char *out;
+    float *lse;
+    int64_t out_row;
+    int nh, hd, type, chunk, lg, n_chunks;
+    int *faults;
+};
+
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs a) {
+    extern __shared__ float lds[];   // [n_chunks] weights, then [groups][hd]
+    __shared__ float red[2 * kJoinThreads / 64];
+    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int i = seq_of_row(a.b, row);
+    if (i >= a.b.n_seqs) return;
+    const Seq s = seq_load(a.b, i);
+    if (!s.fits || row < s.first || row >= s.first + s.rows || s.len <= a.chunk) return;
+    const int nc = (s.len + a.chunk - 1) / a.chunk;
+    const int64_t step = static_cast<int64_t>(a.b.n_rows) * a.nh, at = static_cast<int64_t>(row) * a.nh + head;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ml) + at;
+    float m = -INFINITY;
+    for (int c = tid; c < nc; c += kJoinThreads) m = fmaxf(m, ml[c * step].x);
+    m = wave_max_all_f(m);
+    if (lane == 0) red[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float l = 0.0f;
+    for (int c = tid; c < nc; c += kJoinThreads) {
+        const float2 x = ml[c * step];
+        const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x.x - m) * kLog2e);
+        lds[c] = w;
+        l += x.y * w;
+    }
+    l = wave_sum_f(l);
+    if (lane == 0) red[4 + wave] = l;
+    __syncthreads();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    const int grp = tid / a.lg, groups = kJoinThreads / a.lg, d = 4 * (tid % a.lg);
+    float4 o = float4{0, 0, 0, 0};
+    const float *src = a.parts + at * a.hd + min(d, a.hd - 4);
+#pragma unroll 8
+    for (int c = grp; c < nc; c += groups) {
+        const float4 x = *reinterpret_cast<const float4 *>(src + c * step * a.hd);
+        const float w = lds[c];
+        if (w > 0.0f || w != w) o.x += x.x * w, o.y += x.y * w, o.z += x.z * w, o.w += x.w * w;
+    }
+    float *sum = lds + (a.n_chunks + 3) / 4 * 4;
+    if (d < a.hd) *reinterpret_cast<float4 *>(sum + grp * a.hd + d) = o;
+    __syncthreads();
+    if (grp != 0 || d >= a.hd) return;
+    for (int k = 1; k < groups; ++k) {
+        const float4 x = *reinterpret_cast<const float4 *>(sum + k * a.hd + d);
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+    }
+    const bool some = l > 0.0f || l != l;
+    if (some) o = float4{o.x / l, o.y / l, o.z / l, o.w / l};
+    else o = float4{0, 0, 0, 0};
+    char *dst = a.out + (row * a.out_row + static_cast<int64_t>(head) * a.hd + d) * (a.type == GV_F32 ? 4 : 2);
+    if (a.type == GV_F32) store4<GV_F32>(dst, o);
+    else if (a.type == GV_F16) store4<GV_F16>(dst, o);
+    else store4<GV_BF16>(dst, o);
+    if (a.lse && d == 0) a.lse[at] = some ? m + logf(l) : -INFINITY;
+}
+
+// How a call is cut: column tiles a workgroup takes, groups of them, and positions a chunk. The chunk is the longest of
+// 128 .. 512 that still gives every CU two workgroups over max_len: a short cache is cut fine (its time is latency), and
+// a chunk of 512 writes and reads back a few per cent of the bytes it reads.
+struct AttnPlan {
+    int ct, col_groups, chunk, n_chunks;
+};
+static AttnPlan attn_plan(const gv_paged_kv &kv, const gv_paged_batch &b, int n_heads) {
+    AttnPlan p;
+    const int cols = b.max_rows * (n_heads / kv.n_kv_heads);
+    p.ct = 1;
+    p.col_groups = (cols + 16 * p.ct - 1) / (16 * p.ct);
+    const int64_t items = static_cast<int64_t>(b.n_seqs) * kv.n_kv_heads * p.col_groups;
+    p.chunk = 512;
+    while (p.chunk > 128 && items * ((b.max_len + p.chunk - 1) / p.chunk) < 512) p.chunk /= 2;
+    p.n_chunks = (b.max_len + p.chunk - 1) / p.chunk;
+    return p;
+}
+static size_t attn_ws_bytes(const AttnPlan &p, const gv_paged_kv &kv, const gv_paged_batch &b, int n_heads) {
+    if (p.n_chunks == 1) return 0;
+    return static_cast<size_t>(p.n_chunks) * static_cast<size_t>(b.n_rows) * static_cast<size_t>(n_heads) *
+           (static_cast<size_t>(kv.head_dim) + 2) * 4;
+}
+
+static int check_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, int n_heads, const char *call) {
+    if (check_kv(kv, call) != 0 || check_batch(batch, kv, call) != 0) return -1;
+    GV_CHECK_ARG(batch->max_rows <= kAttnMaxRows, "at most 32 rows a sequence");
+    GV_CHECK_ARG(n_heads >= 1 && n_heads <= 4096 && n_heads % kv->n_kv_heads == 0, "n_heads: a multiple of n_kv_heads, at most 4096");
+    return 0;
+}
+
+}  // namespace gv
+
+using namespace gv;
+
+extern "C" {
+
+size_t gv_paged_attention_workspace_bytes(const gv_paged_kv *kv, const gv_paged_batch *batch, int n_heads) {
+    if (check_attention(kv, batch, n_heads, "gv_paged_attention_workspace_bytes") != 0) return 0;
+    return attn_ws_bytes(attn_plan(*kv, *batch, n_heads), *kv, *batch, n_heads);
+}
+
+int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv_attention_rows *r, void *ws,
+                       size_t ws_bytes) {
+    const char *call = "gv_paged_attention";
+    GV_CHECK_ARG(r, "no rows");
+    if (check_attention(kv, batch, r->n_heads, call) != 0) return -1;
+    GV_CHECK_ARG(float_type(r->type) && (r->type == GV_F32 || r->type == kv->type || kv->type == GV_I8),
+                 "q and out are GV_F32 or the cache's type (GV_I8: any floating type)");
+    const int64_t width = static_cast<int64_t>(r->n_heads) * kv->head_dim, most = int64_t{1} << 36;
+    GV_CHECK_ARG(r->q && r->out && aligned(r->q, 16) && aligned(r->out, 16) && r->q_row >= width && r->out_row >= width &&
+                     r->q_row % 8 == 0 && r->out_row % 8 == 0 && r->q_row < most && r->out_row < most,
+                 "q and out: 16-byte aligned, rows of at least n_heads * head_dim elements, a multiple of 8");
+    GV_CHECK_ARG(r->q != r->out, "out is not q");
+    GV_CHECK_ARG(r->scale == r->scale, "scale is not a number");
+    const AttnPlan p = attn_plan(*kv, *batch, r->n_heads);
+    const size_t need = attn_ws_bytes(p, *kv, *batch, r->n_heads);
+    GV_CHECK_ARG(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need),
+                 "a 16-byte aligned workspace of gv_paged_attention_workspace_bytes");
+    const int64_t units = static_cast<int64_t>(batch->n_seqs) * kv->n_kv_heads * p.n_chunks;
+    const int64_t grid = (units + 7) / 8 * 8 * p.col_groups;
+    GV_CHECK_ARG(grid < int64_t{1} << 31, "too many sequences, heads and positions for one call");
+    if (ensure_init() != 0) return -1;
+    OnDevice dev;
+    int *faults = queued_faults();
+    if (!dev.ok || !faults) return -1;
+    AttnArgs a{};
+    a.kv = kv_view(*kv), a.b = batch_view(*batch);
+    a.q = static_cast<const char *>(r->q), a.out = static_cast<char *>(r->out);
+    a.lse = r->lse, a.visible = r->visible;
+    a.parts = static_cast<float *>(ws);
+    a.ml = need ? a.parts + static_cast<size_t>(p.n_chunks) * batch->n_rows * r->n_heads * kv->head_dim : nullptr;
+    a.q_row = r->q_row, a.out_row = r->out_row;
+    a.nh = r->n_heads, a.group = r->n_heads / kv->n_kv_heads, a.type = r->type;
+    a.chunk = p.chunk, a.n_chunks = p.n_chunks, a.col_groups = p.col_groups;
+    a.scale = r->scale, a.faults = faults;
+    const unsigned g = static_cast<unsigned>(grid);
+    const int rc = kv->type == GV_F16    ? launch_attn_f16(a, p.ct, g, stream())
+                   : kv->type == GV_BF16 ? launch_attn_bf16(a, p.ct, g, stream())
+                                         : launch_attn_i8(a, p.ct, g, stream());
+    if (rc != 0 || p.n_chunks == 1) return rc;
+    JoinArgs j{};
+    j.b = a.b, j.parts = a.parts, j.ml = a.ml, j.out = a.out, j.lse = a.lse, j.out_row = a.out_row;
+    j.nh = a.nh, j.hd = kv->head_dim, j.type = a.type, j.chunk = p.chunk, j.n_chunks = p.n_chunks;
+    j.lg = 4;
+    while (j.lg * 4 < kv->head_dim) j.lg *= 2;
+    const size_t lds = 4 * (static_cast<size_t>((p.n_chunks + 3) / 4 * 4) + static_cast<size_t>(kJoinThreads / j.lg) * kv->head_dim);
+    static int granted = 0;
+    if (lds_grant(reinterpret_cast<const void *>(&paged_join_kernel), lds, granted) != 0) return -1;
+    hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>(batch->n_rows), static_cast<unsigned>(r->n_heads)),
+                       dim3(kJoinThreads), lds, stream(), j);
+    GV_CHECK_HIP(hipGetLastError());
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,600 @@
+// paged_attn.hpp - attention of a few rows a sequence over a paged cache, on the matrix cores. The kernels' template;
+// paged_attn_f16.hip, paged_attn_bf16.hip and paged_attn_i8.hip build it for a cache type each.
+//
+// For a sequence and a KV head, the rows x the query heads that share the head are the columns of S^T = K Q^T (positions
+// x queries) and O^T = V^T P^T (dims x queries). A wave takes 32 positions a step (two tiles of 16, each within a page):
+//   * K tile [16 positions][hd]: a lane's 16-byte loads are MFMA operands as they are (lane: position lane % 16, dims
+//     8 (lane / 16) ..).
+//   * S^T comes out with lane (query lane % 16, positions 4 (lane / 16) .. + 3 of each tile), which is the layout the
+//     second product takes P^T in, when its 8 values a lane are positions {4 g .. 4 g + 3} of the first tile, then of
+//     the second: the weights never leave the registers.
+//   * V rows of those 8 positions: a lane loads NT consecutive dims of each (coalesced over lane % 16) and transposes
+//     the 8 x NT values among its own registers (v_perm_b32, 16-bit pairs): the operand of dim tile n holds dims
+//     {i NT + n}, so no LDS is touched and nothing is stored transposed in the cache.
+// Running maximum and sum a query (fp32); the accumulators are multiplied only in steps where some maximum rose.
+// The four waves of a workgroup take steps in turn over a chunk of positions and are joined in LDS; a sequence of one
+// chunk is finished there, else the chunk's sums go to the workspace and paged_join_kernel (paged_attn.hip) joins them.
+//
+// Rounding: queries and weights go to the matrix cores as PARTS 16-bit parts (fp16: 11 bits each, bf16: 8), keys and
+// values exactly (int8: as fp16 (code) / 512); products are summed in fp32. A query exact in the cache's type is one
+// part; the weights are two parts for 16-bit results (an error of 2^-16 at most, far below the result's own rounding)
+// and 22 or 24 bits for fp32 ones. fp16 parts are taken of values scaled by powers of two (queries by their row's
+// largest value, weights by 2^14), so that neither overflows nor falls below fp16's range.
+// The weights' exponential takes the difference to the maximum: exp2((s - m) log2 e), accurate whatever the scores' size.
+#pragma once
+
+#include "paged.hpp"
+
+namespace gv {
+
+typedef _Float16 ah8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ah2 __attribute__((ext_vector_type(2)));
+typedef __bf16 ab8 __attribute__((ext_vector_type(8)));
+typedef float af4 __attribute__((ext_vector_type(4)));
+typedef uint32_t au4 __attribute__((ext_vector_type(4)));
+
+struct AttnArgs {
+    KvView kv;
+    BatchView b;
+    const char *q;
+    char *out;
+    float *lse;
+    const uint32_t *visible;
+    float *parts, *ml;   // [chunk][row][head][hd] sums, [chunk][row][head][2] (maximum, sum of weights)
+    int64_t q_row, out_row;
+    int nh, group;       // query heads, and those of a KV head
+    int type;            // of q and out
+    int chunk, n_chunks; // positions a workgroup takes; chunks of max_len
+    int col_groups;      // groups of CT x 16 columns that max_rows x group take
+    float scale;
+    int *faults;
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kAttnThreads = 256, kAttnWaves = 4, kAttnStep = 32;
+constexpr int kAttnMaxRows = 32;
+
+// a kernel's LDS: the queries' operands, then (in the same place) the waves' sums of one column tile
+template <int NT, int CT, int QP>
+constexpr int attn_lds() {
+    constexpr int q = CT * QP * (NT / 2) * 64 * 16;
+    constexpr int o = kAttnWaves * 16 * (NT * 16 + 4) * 4;
+    return q > o ? q : o;
+}
+
+__device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+
+// the maximum / sum over the four 16-lane rows, in every lane (each lane keeps its column)
+__device__ inline void rows_pair(float v, int step16, float &a, float &b) {   // v of the two 16-lane rows (halves) of a pair
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = step16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t x = r[0], y = r[1];   // (a vector's element itself is not what a bit cast reads)
+    a = __builtin_bit_cast(float, x), b = __builtin_bit_cast(float, y);
+}
+__device__ inline float rows_max(float v) {
+    float a, b;
+    rows_pair(v, 1, a, b);
+    rows_pair(fmaxf(a, b), 0, a, b);
+    return fmaxf(a, b);
+}
+__device__ inline float rows_sum(float v) {
+    float a, b;
+    rows_pair(v, 1, a, b);
+    rows_pair(a + b, 0, a, b);
+    return a + b;
+}
+
+// N parts of 8 floats in the operand's type: each part the leading bits of what the parts before left (truncated, so
+// that the rest is exact)
+template <bool BF, int N>
+__device__ inline void split8(const float (&x)[8], au4 (&part)[N]) {
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = x[j];
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            if constexpr (BF) {
+                const uint32_t a = __builtin_bit_cast(uint32_t, r[j]), b = __builtin_bit_cast(uint32_t, r[j + 1]);
+                part[p][j / 2] = perm(b, a, 0x07060302u);
+                if (p + 1 < N) {
+                    r[j] -= __builtin_bit_cast(float, a & 0xFFFF0000u);
+                    r[j + 1] -= __builtin_bit_cast(float, b & 0xFFFF0000u);
+                }
+            } else {
+                const auto h = __builtin_amdgcn_cvt_pkrtz(r[j], r[j + 1]);
+                part[p][j / 2] = __builtin_bit_cast(uint32_t, h);
+                if (p + 1 < N) {
+                    r[j] -= static_cast<float>(h[0]);
+                    r[j + 1] -= static_cast<float>(h[1]);
+                }
+            }
+        }
+    }
+}
+
+template <bool BF>
+__device__ inline af4 mfma(au4 a, au4 b, af4 c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ab8, a), __builtin_bit_cast(ab8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ah8, a), __builtin_bit_cast(ah8, b), c, 0, 0, 0);
+}
+
+// bytes (a, b) of two words, each + 128 (their sign bits turned before), as the fp16 pair (a / 512, b / 512): the byte
+// is an fp16 subnormal b 2^-24, times 2^15, minus 128 / 512 (exact)
+__device__ inline uint32_t i8_pair(uint32_t hi, uint32_t lo, uint32_t sel) {
+    const ah2 b = __builtin_bit_cast(ah2, perm(hi, lo, sel));
+    const ah2 v = __builtin_elementwise_fma(b, ah2{static_cast<_Float16>(32768.0f), static_cast<_Float16>(32768.0f)},
+                                            ah2{static_cast<_Float16>(-0.25f), static_cast<_Float16>(-0.25f)});
+    return __builtin_bit_cast(uint32_t, v);
+}
+constexpr float kI8Unit = 512.0f;   // a code's operand x this is the code
+
+// eight consecutive queries' values as floats (TYPE runtime: staging only)
+__device__ inline void load8(const char *p, int type, float (&x)[8]) {
+    if (type == GV_F32) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 16);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const au4 w = *reinterpret_cast<const au4 *>(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[2 * k] = type == GV_F16 ? half_lo(w[k]) : bf16_lo(w[k]);
+            x[2 * k + 1] = type == GV_F16 ? half_hi(w[k]) : bf16_hi(w[k]);
+        }
+    }
+}
+
+// KV: the cache's type. QP, PP: the parts of the queries and of the weights. NT: dim tiles of 16 (head_dim at most
+// 16 NT; EX: exactly). CT: column tiles of 16 queries a workgroup takes.
+template <int KV, int QP, int PP, int NT, bool EX, int CT>
+__global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs a) {
+    constexpr bool BF = KV == GV_BF16, I8 = KV == GV_I8;
+    constexpr int ES = I8 ? 1 : 2;         // bytes a cached element
+    constexpr int NCH = NT / 2;            // 32-dim chunks of S^T's products
+    constexpr int KL = I8 ? NCH / 2 : NCH; // 16-byte loads a lane a K tile
+    constexpr int VW = NT * ES / 4;        // words a lane a V row
+    extern __shared__ au4 lds_q[];         // [CT][QP][NCH][64]
+    __shared__ float lds_amax[CT * 16];
+    __shared__ float lds_m[kAttnWaves][CT * 16], lds_l[kAttnWaves][CT * 16], lds_e[kAttnWaves][CT * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g4 = lane >> 4;
+
+    // which unit: column groups of a (chunk, sequence, KV head) follow each other on one XCD (workgroups go round the
+    // eight), where the second finds the first's keys and values in the L2
+    const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
+    const int cg = idx % a.col_groups;
+    const int64_t unit = static_cast<int64_t>(idx / a.col_groups) * 8 + xcd;
+    const int items = a.b.n_seqs * a.kv.nkv;
+    const int chunk = static_cast<int>(unit / items), item = static_cast<int>(unit % items);
+    if (chunk >= a.n_chunks) return;
+    const int seq = item / a.kv.nkv, head = item % a.kv.nkv;
+    const int p0 = chunk * a.chunk;
+
+    // every load that needs only the sequence at once: its rows and length, and the pages of this wave's tiles (lane t:
+    // step t / 2, tile t % 2; entries past the table's last are not read)
+    const int tile = p0 + kAttnStep * (wave + kAttnWaves * (lane >> 1)) + 16 * (lane & 1);
+    const int64_t entry = tile / a.kv.page;
+    const int page = a.b.pages[seq * a.b.ld_pages + min(entry, static_cast<int64_t>(a.b.max_len - 1) / a.kv.page)];
+    const Seq s = seq_load(a.b, seq);
+    if (!s.fits) {
+        if (threadIdx.x == 0) queue_fault(a.faults, kFaultRows);
+        return;
+    }
+    const int nq = s.rows * a.group, q0 = cg * CT * 16;
+    if (q0 >= nq || p0 >= s.len) return;
+    const int ctx = s.len - s.rows, p1 = min(p0 + a.chunk, s.len);
+    const bool own_tile = tile < p1 && (lane >> 1) * kAttnWaves * kAttnStep < a.chunk;
+    const bool good = page >= 0 && page < a.kv.n_pages;
+    if (own_tile && !good) queue_fault(a.faults, kFaultPage);
+    const bool lost = __any(own_tile && !good);   // (a page outside the pool: its positions read as not seen)
+    const uint64_t usable = __ballot(own_tile && good);
+    const int slot = tile % a.kv.page;
+    const int pg = own_tile && good ? page : 0;
+    const int64_t toff = pg * a.kv.page_stride + head * a.kv.head_stride + slot * a.kv.pos_stride;   // elements
+    const int64_t soff = (static_cast<int64_t>(pg) * a.kv.nkv + head) * a.kv.page + slot;
+
+    // the queries' operands, in the order the products take them: [column tile][part][chunk][lane]
+    for (int i = threadIdx.x; i < CT * 16; i += kAttnThreads) lds_amax[i] = 0.0f;
+    const bool scaled = !BF && a.type != GV_F16;
+    const int qes = a.type == GV_F32 ? 4 : 2;
+    if (scaled) __syncthreads();
+    constexpr int QU = CT * NCH * 64 / kAttnThreads > 0 ? (CT * NCH * 64 + kAttnThreads - 1) / kAttnThreads : 1;
+    float qv[QU][8];
+#pragma unroll
+    for (int u = 0; u < QU; ++u) {
+        const int w = u * kAttnThreads + threadIdx.x, c = w / 64 % NCH, ct = w / 64 / NCH;
+        const int x = q0 + ct * 16 + i16;
+        const int d = I8 ? (c >> 1) * 64 + g4 * 16 + (c & 1) * 8 : c * 32 + g4 * 8;
+        const bool in = ct < CT && x < nq && (EX || d < a.kv.hd);
+        const int xc = in ? x : 0;
+        load8(a.q + ((s.first + xc / a.group) * a.q_row + static_cast<int64_t>(head * a.group + xc % a.group) * a.kv.hd + (in ? d : 0)) * qes,
+              a.type, qv[u]);
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            qv[u][j] = in ? qv[u][j] : 0.0f;
+            m = fmaxf(m, fabsf(qv[u][j]));
+        }
+        // (positive floats order as their bits; an infinity is caught below)
+        if (scaled && in) atomicMax(reinterpret_cast<unsigned *>(lds_amax) + ct * 16 + i16, __float_as_uint(m));
+    }
+    if (scaled) __syncthreads();
+    // a column's power of two: its largest value to 2^10 .. 2^11 (0 and not finite: left)
+    const auto exponent = [&](int ct) {
+        const uint32_t b = __float_as_uint(lds_amax[ct * 16 + i16]);
+        const int e = static_cast<int>(b >> 23);
+        return scaled && e > 0 && e < 255 ? min(max(137 - e, -126), 126) : 0;
+    };
+#pragma unroll
+    for (int u = 0; u < QU; ++u) {
+        const int w = u * kAttnThreads + threadIdx.x, c = w / 64 % NCH, ct = w / 64 / NCH;
+        if (ct >= CT) continue;
+        if (scaled) {
+            const float f = __uint_as_float(static_cast<uint32_t>(127 + exponent(ct)) << 23);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) qv[u][j] *= f;
+        }
+        au4 part[QP];
+        split8<BF, QP>(qv[u], part);
+#pragma unroll
+        for (int p = 0; p < QP; ++p) lds_q[((ct * QP + p) * NCH + c) * 64 + lane] = part[p];
+    }
+    __syncthreads();
+
+    float sc[CT], m[CT], l[CT], ex[CT];   // a column's score factor, maximum, sum; int8: the power of two its weights have
+    uint32_t bits[CT];                    // which of the sequence's rows it sees
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        sc[ct] = a.scale * __uint_as_float(static_cast<uint32_t>(127 - exponent(ct)) << 23) * (I8 ? kI8Unit : 1.0f);
+        m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = 0.0f;
+        const int x = q0 + ct * 16 + i16, r = x / a.group;
+        bits[ct] = x >= nq ? 0u : a.visible ? a.visible[s.first + r] : 0xFFFFFFFFu >> (31 - r);
+    }
+    af4 acc[CT][NT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[ct][n] = af4{0, 0, 0, 0};
+
+    const uint32_t klane = (static_cast<uint32_t>(i16) * static_cast<uint32_t>(a.kv.pos_stride) + g4 * (I8 ? 16 : 8)) * ES;
+    const uint32_t vlane = (static_cast<uint32_t>(4 * g4) * static_cast<uint32_t>(a.kv.pos_stride) + i16 * NT) * ES;
+    const uint32_t vrow = static_cast<uint32_t>(a.kv.pos_stride) * ES;
+    const auto lane64 = [](int64_t v, int l) {
+        const uint64_t u = static_cast<uint64_t>(v);
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u)), l);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u >> 32)), l);
+        return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    };
+
+    for (int st = 0;; ++st) {
+        const int p = p0 + kAttnStep * (wave + kAttnWaves * st);
+        if (p >= p1 || kAttnStep * (kAttnWaves * st) >= a.chunk) break;
+        // ---- loads: both tiles' keys and values (a tile that is not used reads the pool's first page)
+        au4 kf[2][KL];
+        uint32_t vr[8][VW];
+        float ksc[2][4], vsc[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t off = lane64(toff, 2 * st + h);
+            const char *kb = a.kv.k + off * ES;
+#pragma unroll
+            for (int c = 0; c < KL; ++c) {
+                constexpr uint32_t per = I8 ? 64 : 32 * ES;   // bytes between a lane's loads
+                if constexpr (EX) {
+                    kf[h][c] = *reinterpret_cast<const au4 *>(kb + klane + c * per);
+                } else {
+                    const int d = I8 ? c * 64 + g4 * 16 : c * 32 + g4 * 8;
+                    const au4 w = *reinterpret_cast<const au4 *>(kb + (d < a.kv.hd ? klane + c * per : 0));
+                    const uint32_t z = I8 ? 0x00000000u : 0u;
+                    kf[h][c] = d < a.kv.hd ? w : au4{z, z, z, z};
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const char *vb = a.kv.v + lane64(toff, 2 * st + h) * ES;
+            const bool in = EX || i16 * NT < a.kv.hd;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const char *src = vb + (in ? vlane + r * vrow : 0);
+                uint32_t(&w)[VW] = vr[4 * h + r];
+                if constexpr (VW >= 4) {
+#pragma unroll
+                    for (int k = 0; k < VW / 4; ++k) {
+                        const au4 x = *reinterpret_cast<const au4 *>(src + 16 * k);
+                        w[4 * k] = x[0], w[4 * k + 1] = x[1], w[4 * k + 2] = x[2], w[4 * k + 3] = x[3];
+                    }
+                } else if constexpr (VW == 2) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                    w[0] = x.x, w[1] = x.y;
+                } else {
+                    w[0] = *reinterpret_cast<const uint32_t *>(src);
+                }
+            }
+            if constexpr (I8) {
+                const int64_t so = lane64(soff, 2 * st + h) + 4 * g4;
+                const float4 x = *reinterpret_cast<const float4 *>(a.kv.ks + so);
+                const float4 y = *reinterpret_cast<const float4 *>(a.kv.vs + so);
+                ksc[h][0] = x.x, ksc[h][1] = x.y, ksc[h][2] = x.z, ksc[h][3] = x.w;
+                vsc[h][0] = y.x, vsc[h][1] = y.y, vsc[h][2] = y.z, vsc[h][3] = y.w;
+            }
+        }
+
+        // ---- scores
+        af4 sv[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) sv[ct][0] = sv[ct][1] = af4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            au4 kk[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (I8) {
+                    const uint32_t w0 = kf[h][c / 2][2 * (c & 1)] ^ 0x80808080u, w1 = kf[h][c / 2][2 * (c & 1) + 1] ^ 0x80808080u;
+                    kk[h] = au4{i8_pair(0, w0, 0x0C010C00u), i8_pair(0, w0, 0x0C030C02u), i8_pair(0, w1, 0x0C010C00u),
+                                i8_pair(0, w1, 0x0C030C02u)};
+                } else {
+                    kk[h] = kf[h][c];
+                }
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int q = 0; q < QP; ++q) {
+                    const au4 b = lds_q[((ct * QP + q) * NCH + c) * 64 + lane];
+                    sv[ct][0] = mfma<BF>(kk[0], b, sv[ct][0]);
+                    sv[ct][1] = mfma<BF>(kk[1], b, sv[ct][1]);
+                }
+        }
+        // positions that some query does not see: the step reaches the sequence's own rows, its end or a lost page
+        const bool tail = p + kAttnStep > ctx || lost;
+        const bool use0 = usable >> (2 * st) & 1, use1 = usable >> (2 * st + 1) & 1;
+        uint32_t hole = 0;   // (bit j: the lane's position j is not there at all)
+        if (tail) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
+                if (pos >= p1 || !(j < 4 ? use0 : use1)) hole |= 1u << j;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int k = 0; k < VW; ++k) vr[j][k] = hole >> j & 1 ? 0u : vr[j][k];
+        }
+        uint32_t see[CT];   // (bit j: the lane's column sees its position j)
+        au4 pb[CT][PP];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            float x[8], vs[8];
+            see[ct] = 0xFFu;
+            if (tail) {
+                see[ct] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
+                    const bool seen = pos < ctx || (bits[ct] >> ((pos - ctx) & 31) & 1);
+                    if (seen && !(hole >> j & 1)) see[ct] |= 1u << j;
+                }
+            }
+            float top = -INFINITY, vtop = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float f = sc[ct];
+                if constexpr (I8) f *= ksc[j / 4][j % 4], vs[j] = vsc[j / 4][j % 4];
+                x[j] = sv[ct][j / 4][j % 4] * f;
+                if (tail) {
+                    x[j] = see[ct] >> j & 1 ? x[j] : -INFINITY;
+                    if constexpr (I8) vs[j] = see[ct] >> j & 1 ? vs[j] : 0.0f;
+                }
+                top = fmaxf(top, x[j]);
+                if constexpr (I8) vtop = fmaxf(vtop, vs[j]);
+            }
+            top = rows_max(top);
+            if constexpr (I8) {   // the weights' power of two: the largest scale so far below 2
+                vtop = rows_max(vtop);
+                vtop = __uint_as_float(min(__float_as_uint(vtop), 0x7F000000u) & 0x7F800000u);
+            }
+            const float mn = fmaxf(m[ct], top), en = I8 ? fmaxf(ex[ct], vtop) : 0.0f;
+            if (__any(mn > m[ct] || en > ex[ct])) {
+                const float gone = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * kLog2e);
+                l[ct] *= gone;
+                const float f = I8 && en > ex[ct] ? gone * (ex[ct] / en) : gone;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[ct][n] *= f;
+                m[ct] = mn, ex[ct] = en;
+            }
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            const float up = I8 ? (en > 0.0f ? 16384.0f / en : 0.0f) : 16384.0f;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
+                sum += x[j];
+                if constexpr (I8) {
+                    x[j] *= vs[j] * up;
+                    if (tail) x[j] = see[ct] >> j & 1 ? x[j] : 0.0f;
+                } else if constexpr (!BF) {
+                    x[j] *= up;
+                }
+            }
+            l[ct] += sum;
+            split8<BF, PP>(x, pb[ct]);
+        }
+
+        // ---- values: dim tile n's operand from the 8 rows
+        const auto v_tile = [&](int n, uint32_t row_mask) {
+            au4 v;
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+                if constexpr (I8) {
+                    const uint32_t lo = vr[2 * jj][n / 4] ^ 0x80808080u, hi = vr[2 * jj + 1][n / 4] ^ 0x80808080u;
+                    const uint32_t k = n & 3;
+                    v[jj] = i8_pair(hi, lo, 0x0C000C00u | k | (4 + k) << 16);
+                } else {
+                    v[jj] = perm(vr[2 * jj + 1][n / 2], vr[2 * jj][n / 2], n & 1 ? 0x07060302u : 0x05040100u);
+                }
+                if (row_mask != 0xFFu)
+                    v[jj] &= (row_mask >> (2 * jj) & 1 ? 0xFFFFu : 0u) | (row_mask >> (2 * jj + 1) & 1 ? 0xFFFF0000u : 0u);
+            }
+            return v;
+        };
+        // 16-bit values of the sequence's own rows that are not finite reach only the columns that see them: taken out
+        // of the step's product (0 x inf would be NaN), then added position by position to those columns
+        uint32_t wild = 0;
+        if constexpr (!I8) {
+            if (tail) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
+                    bool w = false;
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) {
+                        constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
+                        w |= (vr[j][k] & e) == e || (vr[j][k] >> 16 & e) == e;
+                    }
+                    if (w && pos >= ctx) wild |= 1u << j;
+                }
+            }
+        }
+        const bool any_wild = !I8 && tail && __any(wild != 0);
+        uint32_t rows_in = 0xFFu;
+        if (any_wild) {   // a position is wild for every lane if it is for one of the 16 that hold its dims
+            for (int o = 1; o < 16; o <<= 1) wild |= __shfl_xor(wild, o, 64);
+            rows_in = 0xFFu & ~wild;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const au4 v = v_tile(n, rows_in);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int q = 0; q < PP; ++q) acc[ct][n] = mfma<BF>(v, pb[ct][q], acc[ct][n]);
+            }
+            for (int pp = 0; pp < kAttnStep; ++pp) {   // position pp of the step: lane row pp % 16 / 4, its j
+                const int j = pp / 16 * 4 + pp % 4, g = pp % 16 / 4;
+                if (!(__builtin_amdgcn_readlane(static_cast<int>(wild), 16 * g) >> j & 1)) continue;
+                const uint32_t only = g4 == g ? 1u << j : 0u;
+                uint32_t sees[CT];
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) sees[ct] = __shfl(see[ct], 16 * g + i16, 64) >> j & 1;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const au4 v = v_tile(n, only | 0x100u);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        af4 d = af4{0, 0, 0, 0};
+                        // (the first part alone where the value is infinite: inf - inf of later parts is no number)
+#pragma unroll
+                        for (int q = 0; q < PP; ++q) d = mfma<BF>(v, pb[ct][q], d);
+                        if (sees[ct]) acc[ct][n] += d;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const au4 v = v_tile(n, 0xFFu);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int q = 0; q < PP; ++q) acc[ct][n] = mfma<BF>(v, pb[ct][q], acc[ct][n]);
+            }
+        }
+    }
+
+    // ---- the four waves joined, a column tile after the other
+    constexpr int OLD = NT * 16 + 4;   // floats a column in LDS
+    float *lds_o = reinterpret_cast<float *>(lds_q);
+    __syncthreads();                   // (the queries are done with)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        l[ct] = rows_sum(l[ct]);
+        if (lane < 16) lds_m[wave][ct * 16 + lane] = m[ct], lds_l[wave][ct * 16 + lane] = l[ct], lds_e[wave][ct * 16 + lane] = ex[ct];
+    }
+    __syncthreads();
+    const bool whole = s.len <= a.chunk;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        if (q0 + ct * 16 >= nq) break;
+        const int col = ct * 16 + i16;
+        float mt = lds_m[0][col], et = lds_e[0][col];
+#pragma unroll
+        for (int w = 1; w < kAttnWaves; ++w) mt = fmaxf(mt, lds_m[w][col]), et = fmaxf(et, lds_e[w][col]);
+        float f = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mt) * kLog2e);
+        if constexpr (I8) f = et > 0.0f ? f * (ex[ct] / et) : 0.0f;
+        float *o = lds_o + (wave * 16 + i16) * OLD;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; n += 4)
+                *reinterpret_cast<float4 *>(o + (4 * g4 + r) * NT + n) =
+                    float4{acc[ct][n][r] * f, acc[ct][n + 1][r] * f, acc[ct][n + 2][r] * f, acc[ct][n + 3][r] * f};
+        __syncthreads();
+        for (int u = threadIdx.x; u < 16 * NT * 4; u += kAttnThreads) {
+            const int c = u / (NT * 4), d = u % (NT * 4) * 4;
+            const int x = q0 + ct * 16 + c;
+            if (x >= nq || (!EX && d >= a.kv.hd)) continue;
+            float mm = lds_m[0][ct * 16 + c], ee = lds_e[0][ct * 16 + c];
+#pragma unroll
+            for (int w = 1; w < kAttnWaves; ++w) mm = fmaxf(mm, lds_m[w][ct * 16 + c]), ee = fmaxf(ee, lds_e[w][ct * 16 + c]);
+            float ll = 0.0f;
+            float4 v = float4{0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kAttnWaves; ++w) {
+                const float mw = lds_m[w][ct * 16 + c];
+                if (mw != -INFINITY) ll += lds_l[w][ct * 16 + c] * __builtin_amdgcn_exp2f((mw - mm) * kLog2e);
+                const float4 y = *reinterpret_cast<const float4 *>(lds_o + (w * 16 + c) * OLD + d);
+                v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+            }
+            const int row = s.first + x / a.group, hq = head * a.group + x % a.group;
+            const float unit_v = BF ? 1.0f : I8 ? ee * (kI8Unit / 16384.0f) : 1.0f / 16384.0f;
+            v.x *= unit_v, v.y *= unit_v, v.z *= unit_v, v.w *= unit_v;
+            if (whole) {
+                if (ll > 0.0f || ll != ll) v = float4{v.x / ll, v.y / ll, v.z / ll, v.w / ll};
+                else v = float4{0, 0, 0, 0};
+                char *dst = a.out + (row * a.out_row + static_cast<int64_t>(hq) * a.kv.hd + d) * qes;
+                if (a.type == GV_F32) store4<GV_F32>(dst, v);
+                else if (a.type == GV_F16) store4<GV_F16>(dst, v);
+                else store4<GV_BF16>(dst, v);
+                if (a.lse && d == 0) a.lse[static_cast<int64_t>(row) * a.nh + hq] = ll > 0.0f || ll != ll ? mm + logf(ll) : -INFINITY;
+            } else {
+                const int64_t at = (static_cast<int64_t>(chunk) * a.b.n_rows + row) * a.nh + hq;
+                store4<GV_F32>(reinterpret_cast<char *>(a.parts + at * a.kv.hd + d), v);
+                if (d == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = float2{mm, ll};
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// the kernels of one cache type, by parts (16-bit or fp32 rows), dims and column tiles (paged_attn_<type>.hip)
+int launch_attn_f16(const AttnArgs &a, int ct, unsigned grid, hipStream_t st);
+int launch_attn_bf16(const AttnArgs &a, int ct, unsigned grid, hipStream_t st);
+int launch_attn_i8(const AttnArgs &a, int ct, unsigned grid, hipStream_t st);
+
+template <int KV, int QP, int PP, int NT, bool EX, int CT>
+int launch_attn_one(const AttnArgs &a, unsigned grid, hipStream_t st) {
+    constexpr int lds = attn_lds<NT, CT, QP>();
+    static int granted = 0;
+    if (lds_grant(reinterpret_cast<const void *>(&paged_attn_kernel<KV, QP, PP, NT, EX, CT>), lds, granted) != 0) return -1;
+    hipLaunchKernelGGL((paged_attn_kernel<KV, QP, PP, NT, EX, CT>), dim3(grid), dim3(kAttnThreads), lds, st, a);
+    GV_CHECK_HIP(hipGetLastError());
+    return 0;
+}
+template <int KV, int QP, int PP, int NT, bool EX>
+int launch_attn_ct(const AttnArgs &a, int ct, unsigned grid, hipStream_t st) {
+    (void)ct;
+    return launch_attn_one<KV, QP, PP, NT, EX, 1>(a, grid, st);
+}
+template <int KV, int QP, int PP>
+int launch_attn_nt(const AttnArgs &a, int ct, unsigned grid, hipStream_t st) {
+    switch (a.kv.hd) {
+    case 64: return launch_attn_ct<KV, QP, PP, 4, true>(a, ct, grid, st);
+    case 128: return launch_attn_ct<KV, QP, PP, 8, true>(a, ct, grid, st);
+    case 256: return launch_attn_ct<KV, QP, PP, 16, true>(a, ct, grid, st);
+    }
+    return a.kv.hd < 64 ? launch_attn_ct<KV, QP, PP, 4, false>(a, ct, grid, st)
+           : a.kv.hd < 128 ? launch_attn_ct<KV, QP, PP, 8, false>(a, ct, grid, st)
+                           : launch_attn_ct<KV, QP, PP, 16, false>(a, ct, grid, st);
+}
+
+}  // namespace gv

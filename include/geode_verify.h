@@ -36,6 +36,8 @@ int gv_memcpy_h2d(void *dst, const void *src, size_t bytes);
 int gv_memcpy_d2h(void *dst, const void *src, size_t bytes);
 int gv_memcpy_d2d(void *dst, const void *src, size_t bytes);
 int gv_memset(void *dst, int value, size_t bytes);
+/* Waits for the library's stream. Fails when a call queued since the last one met a fault in device memory (the paged
+ * calls and gv_process_logits below). */
 int gv_synchronize(void);
 /* milliseconds between two points of the library's stream: gv_event_record returns an id */
 int gv_event_record(void);
@@ -383,6 +385,119 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
  * vocabulary, or the top_k / cap candidates) and how many ran the full walks, since the library loaded. No reference
  * counterpart: for tests and measurement, to tell which path served a call. */
 int gv_sampler_paths(int64_t *candidate, int64_t *walks);
+
+/* ------------------------------------------------------------------ several conversations at once
+ * No reference counterpart (the engine serves one conversation over its own contiguous cache, Model::kv): a host that
+ * verifies the rows of several conversations in one step composes it from gv_quantize / gv_gemv_q4 and these calls.
+ * Every array below is device memory of the library's GPU. The calls are enqueued on the library's stream and return
+ * at once: what another stream writes or reads of their arrays has to be ordered against them (gv_synchronize).
+ *
+ * What the host passes is checked by the call (nonzero, gv_last_error). What lies in device memory is checked on the
+ * device: a sequence whose row starts or length do not fit, a page outside the pool, a rotary position outside the
+ * tables, a token range or mask outside its array. Nothing outside the arrays is read or written for it, what it
+ * gives is unspecified, the other sequences and rows are unaffected, and the next gv_synchronize fails with a message. */
+enum { GV_F32 = 0, GV_F16 = 1, GV_BF16 = 2, GV_I8 = 3 }; /* element types */
+
+/* One layer's paged cache: n_pages pages of page_size positions, keys and values apart. The element (page, head,
+ * position, dim) lies at page * page_stride + head * head_stride + position * pos_stride + dim, in k and in v alike, so
+ * positions may lie inside heads or heads inside positions, and k and v may be halves of one page. */
+typedef struct gv_paged_kv {
+    int32_t type;       /* GV_F16, GV_BF16, or GV_I8: int8 with a float scale a (position, KV head), largest / 127, as
+                           the model's int8 cache has (gv_model_config.kv_int8) */
+    int32_t n_kv_heads;
+    int32_t head_dim;   /* a multiple of 16, at most 256 */
+    int32_t page_size;  /* a multiple of 16 */
+    int32_t n_pages;
+    void *k, *v;        /* 16-byte aligned */
+    float *k_scale, *v_scale; /* GV_I8: [n_pages][n_kv_heads][page_size], 16-byte aligned; else ignored */
+    int64_t page_stride, head_stride, pos_stride; /* elements, positive multiples of 16; head_stride and pos_stride below 2^24 */
+} gv_paged_kv;
+
+/* The rows of one step: sequence i has rows row_start[i] .. row_start[i + 1] - 1 (row_start[0] >= 0, never descending;
+ * rows before the first and from row_start[n_seqs] on belong to none and are left as they are) and lens[i] positions in
+ * the cache, its new rows the last of them: its j-th of n rows is position lens[i] - n + j. Position p lies in page
+ * pages[i * ld_pages + p / page_size]; entries past the last position are not read. Sequences may share pages that
+ * no new row goes to. */
+typedef struct gv_paged_batch {
+    int32_t n_seqs, n_rows;  /* n_rows: the rows the step's arrays hold */
+    int32_t max_rows;        /* at least every sequence's rows */
+    int32_t max_len;         /* at least every lens[i]; at most ld_pages * page_size */
+    const int32_t *row_start;/* [n_seqs + 1] */
+    const int32_t *lens;     /* [n_seqs] */
+    const int32_t *pages;    /* [n_seqs][ld_pages] */
+    int64_t ld_pages;
+} gv_paged_batch;
+
+/* New rows to the cache: queries and keys RMSNorm'ed (weight 1 + w, the sum of squares in 64 bits) where a weight is
+ * given, their first rope_dim values rotated, keys and values rounded once to the cache's type, the queries written
+ * to q_out. The model's own arithmetic, value for value (engine/src/model.cpp:3690-3797). */
+typedef struct gv_append_rows {
+    int32_t type;             /* GV_F32, GV_F16 or GV_BF16: q, k and v */
+    int32_t n_heads;          /* query heads, 0: no queries */
+    const void *q, *k, *v;    /* row t's head h at t * q_row + h * q_head (elements, multiples of 4); k, v alike */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* (they may be parts of one array, as q | k | v's product) */
+    const float *q_norm, *k_norm; /* [head_dim] or NULL: not normalized */
+    float eps;
+    int32_t rope_dim;         /* a multiple of 8, at most head_dim; 0: no rotation */
+    int32_t interleaved;      /* 0: value i turns with value i + rope_dim / 2 (the model's); 1: 2 i with 2 i + 1 */
+    const float *cos, *sin;   /* [n_positions][rope_dim / 2] */
+    int32_t n_positions;
+    const int32_t *positions; /* [n_rows] rotary positions (a draft tree's), or NULL: the position in the cache */
+    int32_t q_type;           /* GV_F32, GV_F16 or GV_BF16 */
+    void *q_out;              /* [n_rows], row t's head h at t * q_out_row + h * head_dim; may be q itself, of the same
+                                 type and layout */
+    int64_t q_out_row;
+} gv_append_rows;
+int gv_paged_append(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv_append_rows *rows);
+
+/* Attention of each sequence's rows (at most 32 a sequence) over its cached positions, its own rows' among them:
+ * out = sum softmax(scale q . k) v over the positions before the sequence's first new row and, of its new rows, those
+ * the row sees: itself and the rows before it, or with `visible` the rows j whose bit j is set. A row that sees
+ * nothing gives zeros and lse -inf. What a row does not see does not reach it, NaNs and infinities included. Query head
+ * h reads KV head h / (n_heads / n_kv_heads). Scores, softmax and sums in fp32, the weights with at least 16 bits. */
+typedef struct gv_attention_rows {
+    int32_t type;            /* q and out: the cache's type or GV_F32 (GV_I8: GV_F32, GV_F16 or GV_BF16) */
+    int32_t n_heads;         /* a multiple of n_kv_heads */
+    const void *q;           /* row t's head h at t * q_row + h * head_dim (elements; 16-byte aligned, q_row a multiple of 8) */
+    int64_t q_row;
+    void *out;               /* likewise */
+    int64_t out_row;
+    float *lse;              /* [n_rows][n_heads] log of the sum of exp(score), or NULL */
+    float scale;
+    const uint32_t *visible; /* [n_rows] or NULL: a chain */
+} gv_attention_rows;
+/* Scratch of one call (0: none needed, or arguments that the call refuses). Calls may share it: they run one after
+ * the other. It holds partial results for max_len positions, whatever the lengths turn out to be. */
+size_t gv_paged_attention_workspace_bytes(const gv_paged_kv *kv, const gv_paged_batch *batch, int n_heads);
+int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv_attention_rows *rows, void *ws,
+                       size_t ws_bytes);
+
+/* The rules of each row's request on its logits, before gv_sample_rows or the acceptance calls. Row r's history is
+ * tokens[begin[r] .. end[r]), the request's own part of it from generated[r] on (rows may share ranges: row i of a
+ * draft chain ends i tokens later). In this order, in fp32:
+ *   x = x > 0 ? x / repetition[r] : x * repetition[r]   for the tokens of the history (each once)
+ *   x = x - frequency[r] * (times the token was generated); x = x - presence[r] if it was
+ *   x = x + the sum of the row's biases of the token (in the list's order)
+ *   x = -inf where the row's mask has a zero bit.
+ * Tokens outside [0, V) are ignored. A NULL array: none of its rule. */
+typedef struct gv_logits_rules {
+    const float *repetition, *frequency, *presence; /* [rows] */
+    const int32_t *tokens;
+    int64_t n_tokens;                  /* ranges lie within [0, n_tokens) */
+    const int32_t *begin, *generated, *end; /* [rows]; generated NULL: the whole history */
+    const int32_t *bias_token;
+    const float *bias_value;
+    int64_t n_biases;
+    const int32_t *bias_begin, *bias_end; /* [rows] */
+    const uint32_t *masks;             /* [n_masks][ld_mask], token v's bit v % 32 of word v / 32: 1 stays, 0 goes */
+    int32_t n_masks;
+    int64_t ld_mask;                   /* words, at least ceil(V / 32) */
+    const int32_t *mask_of;            /* [rows] the row's mask, negative: none */
+} gv_logits_rules;
+/* type: GV_F32, GV_F16 or GV_BF16 of the logits; rows ld (out: ldo) elements apart; out may be logits itself
+ * (GV_F32, ldo = ld): what no rule changes is then not written. */
+int gv_process_logits(const gv_logits_rules *rules, const void *logits, int type, int64_t ld, int rows, int V,
+                      float *out, int64_t ldo);
 
 #ifdef __cplusplus
 }
