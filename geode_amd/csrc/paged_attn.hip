@@ -6,24 +6,25 @@
 
 namespace gv {
 
-// A workgroup a (row, query head): the chunks' sums times exp(their maximum - the largest), over the sum of weights.
-// A group of lanes holds a chunk's dims (four a lane), the groups take chunks in turn and are added in LDS.
-// Bound by latency (the row's sequence, the maxima, the sums): the sums were just written and lie in the caches.
-constexpr int kJoinThreads = 256;
+// A workgroup a (row, query head, 64 dims): the chunks' sums times exp(their maximum - the largest), over the sum of
+// weights. 16 groups of 16 lanes (four dims a lane) take chunks in turn, eight in flight each, with a running maximum,
+// and are joined in LDS. Bound by latency (the row's sequence, then the sums, which were just written and lie in the
+// caches): one pass, nothing waits for the overall maximum.
+constexpr int kJoinThreads = 256, kJoinLanes = 16, kJoinGroups = kJoinThreads / kJoinLanes, kJoinDims = 4 * kJoinLanes;
 struct JoinArgs {
     BatchView b;
     const float *parts, *ml;
     char *out;
     float *lse;
     int64_t out_row;
-    int nh, hd, type, chunk, lg, n_chunks;
-    int *faults;
+    int nh, hd, type, chunk;
 };
 
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs a) {
-    extern __shared__ float lds[];   // [n_chunks] weights, then [groups][hd]
-    __shared__ float red[2 * kJoinThreads / 64];
-    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ float4 lds_o[kJoinGroups][kJoinLanes];
+    __shared__ float2 lds_ml[kJoinGroups];
+    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+    const int grp = tid / kJoinLanes, l16 = tid % kJoinLanes, d = blockIdx.z * kJoinDims + 4 * l16;
     const int i = seq_of_row(a.b, row);
     if (i >= a.b.n_seqs) return;
     const Seq s = seq_load(a.b, i);
@@ -31,39 +32,48 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs
     const int nc = (s.len + a.chunk - 1) / a.chunk;
     const int64_t step = static_cast<int64_t>(a.b.n_rows) * a.nh, at = static_cast<int64_t>(row) * a.nh + head;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ml) + at;
-    float m = -INFINITY;
-    for (int c = tid; c < nc; c += kJoinThreads) m = fmaxf(m, ml[c * step].x);
-    m = wave_max_all_f(m);
-    if (lane == 0) red[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float l = 0.0f;
-    for (int c = tid; c < nc; c += kJoinThreads) {
-        const float2 x = ml[c * step];
-        const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x.x - m) * kLog2e);
-        lds[c] = w;
-        l += x.y * w;
-    }
-    l = wave_sum_f(l);
-    if (lane == 0) red[4 + wave] = l;
-    __syncthreads();
-    l = (red[4] + red[5]) + (red[6] + red[7]);
-    const int grp = tid / a.lg, groups = kJoinThreads / a.lg, d = 4 * (tid % a.lg);
-    float4 o = float4{0, 0, 0, 0};
     const float *src = a.parts + at * a.hd + min(d, a.hd - 4);
-#pragma unroll 8
-    for (int c = grp; c < nc; c += groups) {
-        const float4 x = *reinterpret_cast<const float4 *>(src + c * step * a.hd);
-        const float w = lds[c];
-        if (w > 0.0f || w != w) o.x += x.x * w, o.y += x.y * w, o.z += x.z * w, o.w += x.w * w;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = float4{0, 0, 0, 0};
+    constexpr int U = 8;
+    for (int c0 = grp; c0 < nc; c0 += U * kJoinGroups) {
+        float2 x[U];
+        float4 y[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int64_t c = min(c0 + k * kJoinGroups, nc - 1);
+            x[k] = ml[c * step];
+            y[k] = *reinterpret_cast<const float4 *>(src + c * step * a.hd);
+        }
+        float mn = m;
+#pragma unroll
+        for (int k = 0; k < U; ++k) mn = fmaxf(mn, x[k].x);   // (the last chunk again past the end: no harm)
+        if (mn == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f((m - mn) * kLog2e);
+        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f, m = mn;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (c0 + k * kJoinGroups >= nc || x[k].x == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f((x[k].x - m) * kLog2e);
+            l += x[k].y * w;
+            o.x += y[k].x * w, o.y += y[k].y * w, o.z += y[k].z * w, o.w += y[k].w * w;
+        }
     }
-    float *sum = lds + (a.n_chunks + 3) / 4 * 4;
-    if (d < a.hd) *reinterpret_cast<float4 *>(sum + grp * a.hd + d) = o;
+    lds_o[grp][l16] = o;
+    if (l16 == 0) lds_ml[grp] = float2{m, l};
     __syncthreads();
-    if (grp != 0 || d >= a.hd) return;
-    for (int k = 1; k < groups; ++k) {
-        const float4 x = *reinterpret_cast<const float4 *>(sum + k * a.hd + d);
-        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+    if (tid >= kJoinLanes || d >= a.hd) return;
+    m = lds_ml[0].x;
+#pragma unroll
+    for (int g = 1; g < kJoinGroups; ++g) m = fmaxf(m, lds_ml[g].x);
+    l = 0.0f, o = float4{0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < kJoinGroups; ++g) {
+        const float2 x = lds_ml[g];
+        const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x.x - m) * kLog2e);
+        const float4 y = lds_o[g][l16];
+        l += x.y * w;
+        o.x += y.x * w, o.y += y.y * w, o.z += y.z * w, o.w += y.w * w;
     }
     const bool some = l > 0.0f || l != l;
     if (some) o = float4{o.x / l, o.y / l, o.z / l, o.w / l};
@@ -157,14 +167,9 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
     if (rc != 0 || p.n_chunks == 1) return rc;
     JoinArgs j{};
     j.b = a.b, j.parts = a.parts, j.ml = a.ml, j.out = a.out, j.lse = a.lse, j.out_row = a.out_row;
-    j.nh = a.nh, j.hd = kv->head_dim, j.type = a.type, j.chunk = p.chunk, j.n_chunks = p.n_chunks;
-    j.lg = 4;
-    while (j.lg * 4 < kv->head_dim) j.lg *= 2;
-    const size_t lds = 4 * (static_cast<size_t>((p.n_chunks + 3) / 4 * 4) + static_cast<size_t>(kJoinThreads / j.lg) * kv->head_dim);
-    static int granted = 0;
-    if (lds_grant(reinterpret_cast<const void *>(&paged_join_kernel), lds, granted) != 0) return -1;
-    hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>(batch->n_rows), static_cast<unsigned>(r->n_heads)),
-                       dim3(kJoinThreads), lds, stream(), j);
+    j.nh = a.nh, j.hd = kv->head_dim, j.type = a.type, j.chunk = p.chunk;
+    hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>(batch->n_rows), static_cast<unsigned>(r->n_heads),
+                       static_cast<unsigned>((kv->head_dim + kJoinDims - 1) / kJoinDims)), dim3(kJoinThreads), 0, stream(), j);
     GV_CHECK_HIP(hipGetLastError());
     return 0;
 }

@@ -23,6 +23,8 @@
 // The weights' exponential takes the difference to the maximum: exp2((s - m) log2 e), accurate whatever the scores' size.
 #pragma once
 
+#include <type_traits>
+
 #include "paged.hpp"
 
 namespace gv {
@@ -60,6 +62,12 @@ constexpr int attn_lds() {
     constexpr int q = CT * QP * (NT / 2) * 64 * 16;
     constexpr int o = kAttnWaves * 16 * (NT * 16 + 4) * 4;
     return q > o ? q : o;
+}
+
+// waves a SIMD a kernel's registers leave room for (asked of the compiler: more, and it spills)
+template <int KV, int NT, bool EX>
+constexpr int attn_waves() {
+    return NT == 4 ? (KV == GV_I8 && !EX ? 3 : 4) : NT == 8 ? 3 : EX ? 2 : 1;
 }
 
 __device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
@@ -148,7 +156,7 @@ __device__ inline void load8(const char *p, int type, float (&x)[8]) {
 // KV: the cache's type. QP, PP: the parts of the queries and of the weights. NT: dim tiles of 16 (head_dim at most
 // 16 NT; EX: exactly). CT: column tiles of 16 queries a workgroup takes.
 template <int KV, int QP, int PP, int NT, bool EX, int CT>
-__global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void paged_attn_kernel(const AttnArgs a) {
     constexpr bool BF = KV == GV_BF16, I8 = KV == GV_I8;
     constexpr int ES = I8 ? 1 : 2;         // bytes a cached element
     constexpr int NCH = NT / 2;            // 32-dim chunks of S^T's products
@@ -157,7 +165,8 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
     extern __shared__ au4 lds_q[];         // [CT][QP][NCH][64]
     __shared__ float lds_amax[CT * 16];
     __shared__ float lds_m[kAttnWaves][CT * 16], lds_l[kAttnWaves][CT * 16], lds_e[kAttnWaves][CT * 16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g4 = lane >> 4;
+    const int lane = threadIdx.x & 63, i16 = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));   // (uniform: its branches are)
 
     // which unit: column groups of a (chunk, sequence, KV head) follow each other on one XCD (workgroups go round the
     // eight), where the second finds the first's keys and values in the L2
@@ -266,17 +275,14 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
         return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
     };
 
-    for (int st = 0;; ++st) {
-        const int p = p0 + kAttnStep * (wave + kAttnWaves * st);
-        if (p >= p1 || kAttnStep * (kAttnWaves * st) >= a.chunk) break;
-        // ---- loads: both tiles' keys and values (a tile that is not used reads the pool's first page)
-        au4 kf[2][KL];
-        uint32_t vr[8][VW];
-        float ksc[2][4], vsc[2][4];
+    // ---- one step's operands: keys (with their scales) and values; a tile that is not used reads the pool's first page
+    au4 kf[2][KL];
+    uint32_t vr[8][VW];
+    float ksc[2][4], vsc[2][4];
+    const auto load_k = [&](int st) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t off = lane64(toff, 2 * st + h);
-            const char *kb = a.kv.k + off * ES;
+            const char *kb = a.kv.k + lane64(toff, 2 * st + h) * ES;
 #pragma unroll
             for (int c = 0; c < KL; ++c) {
                 constexpr uint32_t per = I8 ? 64 : 32 * ES;   // bytes between a lane's loads
@@ -285,11 +291,16 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
                 } else {
                     const int d = I8 ? c * 64 + g4 * 16 : c * 32 + g4 * 8;
                     const au4 w = *reinterpret_cast<const au4 *>(kb + (d < a.kv.hd ? klane + c * per : 0));
-                    const uint32_t z = I8 ? 0x00000000u : 0u;
-                    kf[h][c] = d < a.kv.hd ? w : au4{z, z, z, z};
+                    kf[h][c] = d < a.kv.hd ? w : au4{0, 0, 0, 0};
                 }
             }
+            if constexpr (I8) {
+                const float4 x = *reinterpret_cast<const float4 *>(a.kv.ks + lane64(soff, 2 * st + h) + 4 * g4);
+                ksc[h][0] = x.x, ksc[h][1] = x.y, ksc[h][2] = x.z, ksc[h][3] = x.w;
+            }
         }
+    };
+    const auto load_v = [&](int st) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const char *vb = a.kv.v + lane64(toff, 2 * st + h) * ES;
@@ -312,14 +323,19 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
                 }
             }
             if constexpr (I8) {
-                const int64_t so = lane64(soff, 2 * st + h) + 4 * g4;
-                const float4 x = *reinterpret_cast<const float4 *>(a.kv.ks + so);
-                const float4 y = *reinterpret_cast<const float4 *>(a.kv.vs + so);
-                ksc[h][0] = x.x, ksc[h][1] = x.y, ksc[h][2] = x.z, ksc[h][3] = x.w;
+                const float4 y = *reinterpret_cast<const float4 *>(a.kv.vs + lane64(soff, 2 * st + h) + 4 * g4);
                 vsc[h][0] = y.x, vsc[h][1] = y.y, vsc[h][2] = y.z, vsc[h][3] = y.w;
             }
         }
+    };
 
+    // One step: the next step's keys are asked for once this one's are in the products, its values likewise. `tail`: a
+    // step with positions that some query does not see (the sequence's own rows, its end, a lost page).
+    const auto step = [&](auto tail_c, int st, bool more) {
+        constexpr bool tail = decltype(tail_c)::value;
+        const int p = p0 + kAttnStep * (wave + kAttnWaves * st);
+        int ql = lane;   // (pinned: the queries are read from LDS in every step, not kept in registers)
+        if constexpr (NT * QP >= 16) asm volatile("" : "+v"(ql));
         // ---- scores
         af4 sv[CT][2];
 #pragma unroll
@@ -341,16 +357,20 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
             for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
                 for (int q = 0; q < QP; ++q) {
-                    const au4 b = lds_q[((ct * QP + q) * NCH + c) * 64 + lane];
+                    const au4 b = lds_q[((ct * QP + q) * NCH + c) * 64 + ql];
                     sv[ct][0] = mfma<BF>(kk[0], b, sv[ct][0]);
                     sv[ct][1] = mfma<BF>(kk[1], b, sv[ct][1]);
                 }
         }
-        // positions that some query does not see: the step reaches the sequence's own rows, its end or a lost page
-        const bool tail = p + kAttnStep > ctx || lost;
+        float kk_sc[8];
+        if constexpr (I8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) kk_sc[j] = ksc[j / 4][j % 4];
+        if constexpr (!tail)
+            if (more) load_k(st + 1);
         const bool use0 = usable >> (2 * st) & 1, use1 = usable >> (2 * st + 1) & 1;
         uint32_t hole = 0;   // (bit j: the lane's position j is not there at all)
-        if (tail) {
+        if constexpr (tail) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
@@ -367,7 +387,7 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
         for (int ct = 0; ct < CT; ++ct) {
             float x[8], vs[8];
             see[ct] = 0xFFu;
-            if (tail) {
+            if constexpr (tail) {
                 see[ct] = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -380,9 +400,9 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float f = sc[ct];
-                if constexpr (I8) f *= ksc[j / 4][j % 4], vs[j] = vsc[j / 4][j % 4];
+                if constexpr (I8) f *= kk_sc[j], vs[j] = vsc[j / 4][j % 4];
                 x[j] = sv[ct][j / 4][j % 4] * f;
-                if (tail) {
+                if constexpr (tail) {
                     x[j] = see[ct] >> j & 1 ? x[j] : -INFINITY;
                     if constexpr (I8) vs[j] = see[ct] >> j & 1 ? vs[j] : 0.0f;
                 }
@@ -412,7 +432,7 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
                 sum += x[j];
                 if constexpr (I8) {
                     x[j] *= vs[j] * up;
-                    if (tail) x[j] = see[ct] >> j & 1 ? x[j] : 0.0f;
+                    if constexpr (tail) x[j] = see[ct] >> j & 1 ? x[j] : 0.0f;
                 } else if constexpr (!BF) {
                     x[j] *= up;
                 }
@@ -422,7 +442,7 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
         }
 
         // ---- values: dim tile n's operand from the 8 rows
-        const auto v_tile = [&](int n, uint32_t row_mask) {
+        const auto v_tile = [&](int n) {
             au4 v;
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
@@ -433,73 +453,82 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(const AttnArgs
                 } else {
                     v[jj] = perm(vr[2 * jj + 1][n / 2], vr[2 * jj][n / 2], n & 1 ? 0x07060302u : 0x05040100u);
                 }
-                if (row_mask != 0xFFu)
-                    v[jj] &= (row_mask >> (2 * jj) & 1 ? 0xFFFFu : 0u) | (row_mask >> (2 * jj + 1) & 1 ? 0xFFFF0000u : 0u);
             }
             return v;
         };
-        // 16-bit values of the sequence's own rows that are not finite reach only the columns that see them: taken out
-        // of the step's product (0 x inf would be NaN), then added position by position to those columns
+        if constexpr (!tail || I8) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const au4 v = v_tile(n);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int q = 0; q < PP; ++q) acc[ct][n] = mfma<BF>(v, pb[ct][q], acc[ct][n]);
+            }
+            if (tail && more) load_k(st + 1);
+            if (more) load_v(st + 1);
+            return;
+        }
+        // 16-bit values of the sequence's own rows that are not finite reach only the columns that see them: left out of
+        // the step's product (0 x inf would be NaN), then added position by position to those columns
         uint32_t wild = 0;
-        if constexpr (!I8) {
-            if (tail) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
-                    bool w = false;
+        for (int j = 0; j < 8; ++j) {
+            const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
+            bool w = false;
 #pragma unroll
-                    for (int k = 0; k < VW; ++k) {
-                        constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
-                        w |= (vr[j][k] & e) == e || (vr[j][k] >> 16 & e) == e;
-                    }
-                    if (w && pos >= ctx) wild |= 1u << j;
-                }
+            for (int k = 0; k < VW; ++k) {
+                constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
+                w |= (vr[j][k] & e) == e || (vr[j][k] >> 16 & e) == e;
             }
+            if (w && pos >= ctx) wild |= 1u << j;
         }
-        const bool any_wild = !I8 && tail && __any(wild != 0);
-        uint32_t rows_in = 0xFFu;
-        if (any_wild) {   // a position is wild for every lane if it is for one of the 16 that hold its dims
+        if (__any(wild != 0))   // wild for every lane if it is for one of the 16 that hold the position's dims
             for (int o = 1; o < 16; o <<= 1) wild |= __shfl_xor(wild, o, 64);
-            rows_in = 0xFFu & ~wild;
+        for (int pp = -1; pp < kAttnStep; ++pp) {   // position pp of the step: lane row pp % 16 / 4, its j
+            const int j = pp < 0 ? 0 : pp / 16 * 4 + pp % 4, g = pp < 0 ? 0 : pp % 16 / 4;
+            if (pp >= 0 && !(__builtin_amdgcn_readlane(static_cast<int>(wild), 16 * g) >> j & 1)) continue;
+            const uint32_t in = pp < 0 ? ~wild : g4 == g ? 1u << j : 0u;
+            uint32_t keep[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) keep[k] = (in >> (2 * k) & 1 ? 0xFFFFu : 0u) | (in >> (2 * k + 1) & 1 ? 0xFFFF0000u : 0u);
+            // (the rows pinned each time round: their transposition would else be kept for all dim tiles at once)
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int k = 0; k < VW; ++k) asm volatile("" : "+v"(vr[r][k]));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const au4 v = v_tile(n, rows_in);
+                au4 v = v_tile(n);
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
+                for (int k = 0; k < 4; ++k) v[k] &= keep[k];
 #pragma unroll
-                    for (int q = 0; q < PP; ++q) acc[ct][n] = mfma<BF>(v, pb[ct][q], acc[ct][n]);
-            }
-            for (int pp = 0; pp < kAttnStep; ++pp) {   // position pp of the step: lane row pp % 16 / 4, its j
-                const int j = pp / 16 * 4 + pp % 4, g = pp % 16 / 4;
-                if (!(__builtin_amdgcn_readlane(static_cast<int>(wild), 16 * g) >> j & 1)) continue;
-                const uint32_t only = g4 == g ? 1u << j : 0u;
-                uint32_t sees[CT];
+                for (int ct = 0; ct < CT; ++ct) {
+                    af4 d = af4{0, 0, 0, 0};
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) sees[ct] = __shfl(see[ct], 16 * g + i16, 64) >> j & 1;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const au4 v = v_tile(n, only | 0x100u);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        af4 d = af4{0, 0, 0, 0};
-                        // (the first part alone where the value is infinite: inf - inf of later parts is no number)
-#pragma unroll
-                        for (int q = 0; q < PP; ++q) d = mfma<BF>(v, pb[ct][q], d);
-                        if (sees[ct]) acc[ct][n] += d;
-                    }
+                    for (int q = 0; q < PP; ++q) d = mfma<BF>(v, pb[ct][q], d);
+                    const bool sees = pp < 0 || (__shfl(see[ct], 16 * g + i16, 64) >> j & 1);
+                    if (sees) acc[ct][n] += d;
                 }
             }
-        } else {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const au4 v = v_tile(n, 0xFFu);
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                    for (int q = 0; q < PP; ++q) acc[ct][n] = mfma<BF>(v, pb[ct][q], acc[ct][n]);
-            }
+            if (!__any(wild != 0)) break;
         }
+        if (more) {
+            load_k(st + 1);
+            load_v(st + 1);
+        }
+    };
+    const int mine = p1 - p0 - kAttnStep * wave, open = ctx - p0 - kAttnStep * (wave + 1);
+    constexpr int kRound = kAttnStep * kAttnWaves;
+    const int steps = mine > 0 ? (mine + kRound - 1) / kRound : 0;
+    const int free_steps = lost || open < 0 ? 0 : min(steps, open / kRound + 1);
+    if (steps > 0) {
+        load_k(0);
+        load_v(0);
     }
+    int st = 0;
+    for (; st < free_steps; ++st) step(std::false_type{}, st, st + 1 < steps);
+    for (; st < steps; ++st) step(std::true_type{}, st, st + 1 < steps);
 
     // ---- the four waves joined, a column tile after the other
     constexpr int OLD = NT * 16 + 4;   // floats a column in LDS
