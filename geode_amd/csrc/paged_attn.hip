@@ -7,7 +7,7 @@
 namespace gv {
 
 // A workgroup a (row, query head, 64 dims): the chunks' sums times exp(their maximum - the largest), over the sum of
-// weights. 16 groups of 16 lanes (four dims a lane) take chunks in turn, eight in flight each, with a running maximum,
+// weights. 16 groups of 16 lanes (four dims a lane) take chunks in turn, one to eight in flight each, with a running maximum,
 // and are joined in LDS. Bound by latency (the row's sequence, then the sums, which were just written and lie in the
 // caches): one pass, nothing waits for the overall maximum.
 constexpr int kJoinThreads = 256, kJoinLanes = 16, kJoinGroups = kJoinThreads / kJoinLanes, kJoinDims = 4 * kJoinLanes;
@@ -23,11 +23,11 @@ struct JoinArgs {
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs a) {
     __shared__ float4 lds_o[kJoinGroups][kJoinLanes];
     __shared__ float2 lds_ml[kJoinGroups];
+    touch_args(a);
     const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
     const int grp = tid / kJoinLanes, l16 = tid % kJoinLanes, d = blockIdx.z * kJoinDims + 4 * l16;
-    const int i = seq_of_row(a.b, row);
-    if (i >= a.b.n_seqs) return;
-    const Seq s = seq_load(a.b, i);
+    Seq s;
+    if (seq_of_row(a.b, row, s) >= a.b.n_seqs) return;
     if (!s.fits || row < s.first || row >= s.first + s.rows || s.len <= a.chunk) return;
     const int nc = (s.len + a.chunk - 1) / a.chunk;
     const int64_t step = static_cast<int64_t>(a.b.n_rows) * a.nh, at = static_cast<int64_t>(row) * a.nh + head;
@@ -35,30 +35,35 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs
     const float *src = a.parts + at * a.hd + min(d, a.hd - 4);
     float m = -INFINITY, l = 0.0f;
     float4 o = float4{0, 0, 0, 0};
-    constexpr int U = 8;
-    for (int c0 = grp; c0 < nc; c0 += U * kJoinGroups) {
-        float2 x[U];
-        float4 y[U];
+    const auto take = [&](auto in_flight) {
+        constexpr int U = decltype(in_flight)::value;
+        for (int c0 = grp; c0 < nc; c0 += U * kJoinGroups) {
+            float2 x[U];
+            float4 y[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const int64_t c = min(c0 + k * kJoinGroups, nc - 1);
-            x[k] = ml[c * step];
-            y[k] = *reinterpret_cast<const float4 *>(src + c * step * a.hd);
+            for (int k = 0; k < U; ++k) {
+                const int64_t c = min(c0 + k * kJoinGroups, nc - 1);
+                x[k] = ml[c * step];
+                y[k] = *reinterpret_cast<const float4 *>(src + c * step * a.hd);
+            }
+            float mn = m;
+#pragma unroll
+            for (int k = 0; k < U; ++k) mn = fmaxf(mn, x[k].x);   // (the last chunk again past the end: no harm)
+            if (mn == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f((m - mn) * kLog2e);
+            l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f, m = mn;
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                if (c0 + k * kJoinGroups >= nc || x[k].x == -INFINITY) continue;
+                const float w = __builtin_amdgcn_exp2f((x[k].x - m) * kLog2e);
+                l += x[k].y * w;
+                o.x += y[k].x * w, o.y += y[k].y * w, o.z += y[k].z * w, o.w += y[k].w * w;
+            }
         }
-        float mn = m;
-#pragma unroll
-        for (int k = 0; k < U; ++k) mn = fmaxf(mn, x[k].x);   // (the last chunk again past the end: no harm)
-        if (mn == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f((m - mn) * kLog2e);
-        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f, m = mn;
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            if (c0 + k * kJoinGroups >= nc || x[k].x == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f((x[k].x - m) * kLog2e);
-            l += x[k].y * w;
-            o.x += y[k].x * w, o.y += y[k].y * w, o.z += y[k].z * w, o.w += y[k].w * w;
-        }
-    }
+    };
+    if (nc <= kJoinGroups) take(std::integral_constant<int, 1>{});
+    else if (nc <= 4 * kJoinGroups) take(std::integral_constant<int, 4>{});
+    else take(std::integral_constant<int, 8>{});
     lds_o[grp][l16] = o;
     if (l16 == 0) lds_ml[grp] = float2{m, l};
     __syncthreads();

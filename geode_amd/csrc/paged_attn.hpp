@@ -56,17 +56,25 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kAttnThreads = 256, kAttnWaves = 4, kAttnStep = 32;
 constexpr int kAttnMaxRows = 32;
 
+// Many columns of long rows: the sums of three column tiles x 256 dims would take 192 registers of a wave. Two waves then
+// share a step's positions and take half the dims of O^T each (both make the scores: the second's keys come from the
+// caches, and the matrix cores have the time).
+template <int NT, int CT>
+constexpr int attn_dim_split() {
+    return NT == 16 && CT > 1 ? 2 : 1;
+}
 // a kernel's LDS: the queries' operands, then (in the same place) the waves' sums of one column tile
 template <int NT, int CT, int QP>
 constexpr int attn_lds() {
     constexpr int q = CT * QP * (NT / 2) * 64 * 16;
-    constexpr int o = kAttnWaves * 16 * (NT * 16 + 4) * 4;
+    constexpr int o = kAttnWaves / attn_dim_split<NT, CT>() * 16 * (NT * 16 + 4) * 4;
     return q > o ? q : o;
 }
 
 // waves a SIMD a kernel's registers leave room for (asked of the compiler: more, and it spills)
-template <int KV, int NT, bool EX>
+template <int KV, int NT, bool EX, int CT>
 constexpr int attn_waves() {
+    if (CT > 1) return NT == 4 ? 2 : 1;
     return NT == 4 ? (KV == GV_I8 && !EX ? 3 : 4) : NT == 8 ? 3 : EX ? 2 : 1;
 }
 
@@ -156,17 +164,20 @@ __device__ inline void load8(const char *p, int type, float (&x)[8]) {
 // KV: the cache's type. QP, PP: the parts of the queries and of the weights. NT: dim tiles of 16 (head_dim at most
 // 16 NT; EX: exactly). CT: column tiles of 16 queries a workgroup takes.
 template <int KV, int QP, int PP, int NT, bool EX, int CT>
-__global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void paged_attn_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void paged_attn_kernel(const AttnArgs a) {
     constexpr bool BF = KV == GV_BF16, I8 = KV == GV_I8;
     constexpr int ES = I8 ? 1 : 2;         // bytes a cached element
     constexpr int NCH = NT / 2;            // 32-dim chunks of S^T's products
     constexpr int KL = I8 ? NCH / 2 : NCH; // 16-byte loads a lane a K tile
-    constexpr int VW = NT * ES / 4;        // words a lane a V row
+    constexpr int DS = attn_dim_split<NT, CT>(), NV = NT / DS, PW = kAttnWaves / DS;   // (see there)
+    constexpr int VW = NV * ES / 4;        // words a lane a V row
     extern __shared__ au4 lds_q[];         // [CT][QP][NCH][64]
     __shared__ float lds_amax[CT * 16];
-    __shared__ float lds_m[kAttnWaves][CT * 16], lds_l[kAttnWaves][CT * 16], lds_e[kAttnWaves][CT * 16];
+    __shared__ float lds_m[PW][CT * 16], lds_l[PW][CT * 16], lds_e[PW][CT * 16];
+    touch_args(a);
     const int lane = threadIdx.x & 63, i16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));   // (uniform: its branches are)
+    const int pw = wave / DS, half = wave % DS;   // whose positions, which dims
 
     // which unit: column groups of a (chunk, sequence, KV head) follow each other on one XCD (workgroups go round the
     // eight), where the second finds the first's keys and values in the L2
@@ -181,7 +192,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
 
     // every load that needs only the sequence at once: its rows and length, and the pages of this wave's tiles (lane t:
     // step t / 2, tile t % 2; entries past the table's last are not read)
-    const int tile = p0 + kAttnStep * (wave + kAttnWaves * (lane >> 1)) + 16 * (lane & 1);
+    const int tile = p0 + kAttnStep * (pw + PW * (lane >> 1)) + 16 * (lane & 1);
     const int64_t entry = tile / a.kv.page;
     const int page = a.b.pages[seq * a.b.ld_pages + min(entry, static_cast<int64_t>(a.b.max_len - 1) / a.kv.page)];
     const Seq s = seq_load(a.b, seq);
@@ -192,7 +203,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
     const int nq = s.rows * a.group, q0 = cg * CT * 16;
     if (q0 >= nq || p0 >= s.len) return;
     const int ctx = s.len - s.rows, p1 = min(p0 + a.chunk, s.len);
-    const bool own_tile = tile < p1 && (lane >> 1) * kAttnWaves * kAttnStep < a.chunk;
+    const bool own_tile = tile < p1 && (lane >> 1) * PW * kAttnStep < a.chunk;
     const bool good = page >= 0 && page < a.kv.n_pages;
     if (own_tile && !good) queue_fault(a.faults, kFaultPage);
     const bool lost = __any(own_tile && !good);   // (a page outside the pool: its positions read as not seen)
@@ -201,6 +212,80 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
     const int pg = own_tile && good ? page : 0;
     const int64_t toff = pg * a.kv.page_stride + head * a.kv.head_stride + slot * a.kv.pos_stride;   // elements
     const int64_t soff = (static_cast<int64_t>(pg) * a.kv.nkv + head) * a.kv.page + slot;
+
+    const uint32_t klane = (static_cast<uint32_t>(i16) * static_cast<uint32_t>(a.kv.pos_stride) + g4 * (I8 ? 16 : 8)) * ES;
+    const int vdim = half * NV * 16 + i16 * NV;   // the lane's first dim of the values
+    const uint32_t vlane = (static_cast<uint32_t>(4 * g4) * static_cast<uint32_t>(a.kv.pos_stride) + vdim) * ES;
+    const uint32_t vrow = static_cast<uint32_t>(a.kv.pos_stride) * ES;
+    const auto lane64 = [](int64_t v, int l) {
+        const uint64_t u = static_cast<uint64_t>(v);
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u)), l);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u >> 32)), l);
+        return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    };
+
+    // ---- one step's operands: keys (with their scales) and values; a tile that is not used reads the pool's first page
+    au4 kf[2][KL];
+    uint32_t vr[8][VW];
+    float ksc[2][4], vsc[2][4];
+    const auto load_k = [&](int st) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const char *kb = a.kv.k + lane64(toff, 2 * st + h) * ES;
+#pragma unroll
+            for (int c = 0; c < KL; ++c) {
+                constexpr uint32_t per = I8 ? 64 : 32 * ES;   // bytes between a lane's loads
+                if constexpr (EX) {
+                    kf[h][c] = *reinterpret_cast<const au4 *>(kb + klane + c * per);
+                } else {
+                    const int d = I8 ? c * 64 + g4 * 16 : c * 32 + g4 * 8;
+                    const au4 w = *reinterpret_cast<const au4 *>(kb + (d < a.kv.hd ? klane + c * per : 0));
+                    kf[h][c] = d < a.kv.hd ? w : au4{0, 0, 0, 0};
+                }
+            }
+            if constexpr (I8) {
+                const float4 x = *reinterpret_cast<const float4 *>(a.kv.ks + lane64(soff, 2 * st + h) + 4 * g4);
+                ksc[h][0] = x.x, ksc[h][1] = x.y, ksc[h][2] = x.z, ksc[h][3] = x.w;
+            }
+        }
+    };
+    const auto load_v = [&](int st) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const char *vb = a.kv.v + lane64(toff, 2 * st + h) * ES;
+            const bool in = EX || vdim < a.kv.hd;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const char *src = vb + (in ? vlane + r * vrow : 0);
+                uint32_t(&w)[VW] = vr[4 * h + r];
+                if constexpr (VW >= 4) {
+#pragma unroll
+                    for (int k = 0; k < VW / 4; ++k) {
+                        const au4 x = *reinterpret_cast<const au4 *>(src + 16 * k);
+                        w[4 * k] = x[0], w[4 * k + 1] = x[1], w[4 * k + 2] = x[2], w[4 * k + 3] = x[3];
+                    }
+                } else if constexpr (VW == 2) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                    w[0] = x.x, w[1] = x.y;
+                } else {
+                    w[0] = *reinterpret_cast<const uint32_t *>(src);
+                }
+            }
+            if constexpr (I8) {
+                const float4 y = *reinterpret_cast<const float4 *>(a.kv.vs + lane64(soff, 2 * st + h) + 4 * g4);
+                vsc[h][0] = y.x, vsc[h][1] = y.y, vsc[h][2] = y.z, vsc[h][3] = y.w;
+            }
+        }
+    };
+
+    const int mine = p1 - p0 - kAttnStep * pw, open = ctx - p0 - kAttnStep * (pw + 1);
+    constexpr int kRound = kAttnStep * PW;
+    const int steps = mine > 0 ? (mine + kRound - 1) / kRound : 0;
+    const int free_steps = lost || open < 0 ? 0 : min(steps, open / kRound + 1);
+    if (steps > 0) {   // (the first step's keys and values on their way while the queries are made ready)
+        load_k(0);
+        load_v(0);
+    }
 
     // the queries' operands, in the order the products take them: [column tile][part][chunk][lane]
     for (int i = threadIdx.x; i < CT * 16; i += kAttnThreads) lds_amax[i] = 0.0f;
@@ -259,83 +344,19 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
         const int x = q0 + ct * 16 + i16, r = x / a.group;
         bits[ct] = x >= nq ? 0u : a.visible ? a.visible[s.first + r] : 0xFFFFFFFFu >> (31 - r);
     }
-    af4 acc[CT][NT];
+    af4 acc[CT][NV];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[ct][n] = af4{0, 0, 0, 0};
-
-    const uint32_t klane = (static_cast<uint32_t>(i16) * static_cast<uint32_t>(a.kv.pos_stride) + g4 * (I8 ? 16 : 8)) * ES;
-    const uint32_t vlane = (static_cast<uint32_t>(4 * g4) * static_cast<uint32_t>(a.kv.pos_stride) + i16 * NT) * ES;
-    const uint32_t vrow = static_cast<uint32_t>(a.kv.pos_stride) * ES;
-    const auto lane64 = [](int64_t v, int l) {
-        const uint64_t u = static_cast<uint64_t>(v);
-        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u)), l);
-        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u >> 32)), l);
-        return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-    };
-
-    // ---- one step's operands: keys (with their scales) and values; a tile that is not used reads the pool's first page
-    au4 kf[2][KL];
-    uint32_t vr[8][VW];
-    float ksc[2][4], vsc[2][4];
-    const auto load_k = [&](int st) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const char *kb = a.kv.k + lane64(toff, 2 * st + h) * ES;
-#pragma unroll
-            for (int c = 0; c < KL; ++c) {
-                constexpr uint32_t per = I8 ? 64 : 32 * ES;   // bytes between a lane's loads
-                if constexpr (EX) {
-                    kf[h][c] = *reinterpret_cast<const au4 *>(kb + klane + c * per);
-                } else {
-                    const int d = I8 ? c * 64 + g4 * 16 : c * 32 + g4 * 8;
-                    const au4 w = *reinterpret_cast<const au4 *>(kb + (d < a.kv.hd ? klane + c * per : 0));
-                    kf[h][c] = d < a.kv.hd ? w : au4{0, 0, 0, 0};
-                }
-            }
-            if constexpr (I8) {
-                const float4 x = *reinterpret_cast<const float4 *>(a.kv.ks + lane64(soff, 2 * st + h) + 4 * g4);
-                ksc[h][0] = x.x, ksc[h][1] = x.y, ksc[h][2] = x.z, ksc[h][3] = x.w;
-            }
-        }
-    };
-    const auto load_v = [&](int st) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const char *vb = a.kv.v + lane64(toff, 2 * st + h) * ES;
-            const bool in = EX || i16 * NT < a.kv.hd;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const char *src = vb + (in ? vlane + r * vrow : 0);
-                uint32_t(&w)[VW] = vr[4 * h + r];
-                if constexpr (VW >= 4) {
-#pragma unroll
-                    for (int k = 0; k < VW / 4; ++k) {
-                        const au4 x = *reinterpret_cast<const au4 *>(src + 16 * k);
-                        w[4 * k] = x[0], w[4 * k + 1] = x[1], w[4 * k + 2] = x[2], w[4 * k + 3] = x[3];
-                    }
-                } else if constexpr (VW == 2) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
-                    w[0] = x.x, w[1] = x.y;
-                } else {
-                    w[0] = *reinterpret_cast<const uint32_t *>(src);
-                }
-            }
-            if constexpr (I8) {
-                const float4 y = *reinterpret_cast<const float4 *>(a.kv.vs + lane64(soff, 2 * st + h) + 4 * g4);
-                vsc[h][0] = y.x, vsc[h][1] = y.y, vsc[h][2] = y.z, vsc[h][3] = y.w;
-            }
-        }
-    };
+        for (int n = 0; n < NV; ++n) acc[ct][n] = af4{0, 0, 0, 0};
 
     // One step: the next step's keys are asked for once this one's are in the products, its values likewise. `tail`: a
     // step with positions that some query does not see (the sequence's own rows, its end, a lost page).
     const auto step = [&](auto tail_c, int st, bool more) {
         constexpr bool tail = decltype(tail_c)::value;
-        const int p = p0 + kAttnStep * (wave + kAttnWaves * st);
+        const int p = p0 + kAttnStep * (pw + PW * st);
         int ql = lane;   // (pinned: the queries are read from LDS in every step, not kept in registers)
-        if constexpr (NT * QP >= 16) asm volatile("" : "+v"(ql));
+        if constexpr (CT * NT * QP >= 16) asm volatile("" : "+v"(ql));
         // ---- scores
         af4 sv[CT][2];
 #pragma unroll
@@ -420,7 +441,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
                 l[ct] *= gone;
                 const float f = I8 && en > ex[ct] ? gone * (ex[ct] / en) : gone;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) acc[ct][n] *= f;
+                for (int n = 0; n < NV; ++n) acc[ct][n] *= f;
                 m[ct] = mn, ex[ct] = en;
             }
             const float base = mn == -INFINITY ? 0.0f : mn;
@@ -458,7 +479,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
         };
         if constexpr (!tail || I8) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < NV; ++n) {
                 const au4 v = v_tile(n);
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
@@ -498,7 +519,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
 #pragma unroll
                 for (int k = 0; k < VW; ++k) asm volatile("" : "+v"(vr[r][k]));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < NV; ++n) {
                 au4 v = v_tile(n);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] &= keep[k];
@@ -518,14 +539,6 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
             load_v(st + 1);
         }
     };
-    const int mine = p1 - p0 - kAttnStep * wave, open = ctx - p0 - kAttnStep * (wave + 1);
-    constexpr int kRound = kAttnStep * kAttnWaves;
-    const int steps = mine > 0 ? (mine + kRound - 1) / kRound : 0;
-    const int free_steps = lost || open < 0 ? 0 : min(steps, open / kRound + 1);
-    if (steps > 0) {
-        load_k(0);
-        load_v(0);
-    }
     int st = 0;
     for (; st < free_steps; ++st) step(std::false_type{}, st, st + 1 < steps);
     for (; st < steps; ++st) step(std::true_type{}, st, st + 1 < steps);
@@ -537,7 +550,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         l[ct] = rows_sum(l[ct]);
-        if (lane < 16) lds_m[wave][ct * 16 + lane] = m[ct], lds_l[wave][ct * 16 + lane] = l[ct], lds_e[wave][ct * 16 + lane] = ex[ct];
+        if (half == 0 && lane < 16) lds_m[pw][ct * 16 + lane] = m[ct], lds_l[pw][ct * 16 + lane] = l[ct], lds_e[pw][ct * 16 + lane] = ex[ct];
     }
     __syncthreads();
     const bool whole = s.len <= a.chunk;
@@ -547,15 +560,15 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
         const int col = ct * 16 + i16;
         float mt = lds_m[0][col], et = lds_e[0][col];
 #pragma unroll
-        for (int w = 1; w < kAttnWaves; ++w) mt = fmaxf(mt, lds_m[w][col]), et = fmaxf(et, lds_e[w][col]);
+        for (int w = 1; w < PW; ++w) mt = fmaxf(mt, lds_m[w][col]), et = fmaxf(et, lds_e[w][col]);
         float f = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mt) * kLog2e);
         if constexpr (I8) f = et > 0.0f ? f * (ex[ct] / et) : 0.0f;
-        float *o = lds_o + (wave * 16 + i16) * OLD;
+        float *o = lds_o + (pw * 16 + i16) * OLD + half * NV * 16;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int n = 0; n < NT; n += 4)
-                *reinterpret_cast<float4 *>(o + (4 * g4 + r) * NT + n) =
+            for (int n = 0; n < NV; n += 4)
+                *reinterpret_cast<float4 *>(o + (4 * g4 + r) * NV + n) =
                     float4{acc[ct][n][r] * f, acc[ct][n + 1][r] * f, acc[ct][n + 2][r] * f, acc[ct][n + 3][r] * f};
         __syncthreads();
         for (int u = threadIdx.x; u < 16 * NT * 4; u += kAttnThreads) {
@@ -564,11 +577,11 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX>())) void page
             if (x >= nq || (!EX && d >= a.kv.hd)) continue;
             float mm = lds_m[0][ct * 16 + c], ee = lds_e[0][ct * 16 + c];
 #pragma unroll
-            for (int w = 1; w < kAttnWaves; ++w) mm = fmaxf(mm, lds_m[w][ct * 16 + c]), ee = fmaxf(ee, lds_e[w][ct * 16 + c]);
+            for (int w = 1; w < PW; ++w) mm = fmaxf(mm, lds_m[w][ct * 16 + c]), ee = fmaxf(ee, lds_e[w][ct * 16 + c]);
             float ll = 0.0f;
             float4 v = float4{0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) {
+            for (int w = 0; w < PW; ++w) {
                 const float mw = lds_m[w][ct * 16 + c];
                 if (mw != -INFINITY) ll += lds_l[w][ct * 16 + c] * __builtin_amdgcn_exp2f((mw - mm) * kLog2e);
                 const float4 y = *reinterpret_cast<const float4 *>(lds_o + (w * 16 + c) * OLD + d);
@@ -611,8 +624,7 @@ int launch_attn_one(const AttnArgs &a, unsigned grid, hipStream_t st) {
 }
 template <int KV, int QP, int PP, int NT, bool EX>
 int launch_attn_ct(const AttnArgs &a, int ct, unsigned grid, hipStream_t st) {
-    (void)ct;
-    return launch_attn_one<KV, QP, PP, NT, EX, 1>(a, grid, st);
+    return ct == 1 ? launch_attn_one<KV, QP, PP, NT, EX, 1>(a, grid, st) : launch_attn_one<KV, QP, PP, NT, EX, 3>(a, grid, st);
 }
 template <int KV, int QP, int PP>
 int launch_attn_nt(const AttnArgs &a, int ct, unsigned grid, hipStream_t st) {

@@ -477,13 +477,13 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
  * draft chain ends i tokens later). In this order, in fp32:
  *   x = x > 0 ? x / repetition[r] : x * repetition[r]   for the tokens of the history (each once)
  *   x = x - frequency[r] * (times the token was generated); x = x - presence[r] if it was
- *   x = x + the sum of the row's biases of the token (in the list's order)
+ *   x = x + the row's biases of the token, one after the other in the list's order
  *   x = -inf where the row's mask has a zero bit.
  * Tokens outside [0, V) are ignored. A NULL array: none of its rule. */
 typedef struct gv_logits_rules {
     const float *repetition, *frequency, *presence; /* [rows] */
     const int32_t *tokens;
-    int64_t n_tokens;                  /* ranges lie within [0, n_tokens) */
+    int64_t n_tokens;                  /* ranges lie within [0, n_tokens); at most 2^30 */
     const int32_t *begin, *generated, *end; /* [rows]; generated NULL: the whole history */
     const int32_t *bias_token;
     const float *bias_value;
