@@ -7,10 +7,10 @@
 namespace gv {
 
 // A workgroup a (row, query head, 64 dims): the chunks' sums times exp(their maximum - the largest), over the sum of
-// weights. 16 groups of 16 lanes (four dims a lane) take chunks in turn, one to eight in flight each, with a running maximum,
+// weights. 4 or 16 groups of 16 lanes (four dims a lane) take chunks in turn, one to eight in flight each, with a running maximum,
 // and are joined in LDS. Bound by latency (the row's sequence, then the sums, which were just written and lie in the
 // caches): one pass, nothing waits for the overall maximum.
-constexpr int kJoinThreads = 256, kJoinLanes = 16, kJoinGroups = kJoinThreads / kJoinLanes, kJoinDims = 4 * kJoinLanes;
+constexpr int kJoinLanes = 16, kJoinDims = 4 * kJoinLanes;
 struct JoinArgs {
     BatchView b;
     const float *parts, *ml;
@@ -20,9 +20,10 @@ struct JoinArgs {
     int nh, hd, type, chunk;
 };
 
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs a) {
-    __shared__ float4 lds_o[kJoinGroups][kJoinLanes];
-    __shared__ float2 lds_ml[kJoinGroups];
+template <int GROUPS>
+__global__ __launch_bounds__(GROUPS * kJoinLanes) void paged_join_kernel(const JoinArgs a) {
+    __shared__ float4 lds_o[GROUPS][kJoinLanes];
+    __shared__ float2 lds_ml[GROUPS];
     touch_args(a);
     const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
     const int grp = tid / kJoinLanes, l16 = tid % kJoinLanes, d = blockIdx.z * kJoinDims + 4 * l16;
@@ -37,12 +38,12 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs
     float4 o = float4{0, 0, 0, 0};
     const auto take = [&](auto in_flight) {
         constexpr int U = decltype(in_flight)::value;
-        for (int c0 = grp; c0 < nc; c0 += U * kJoinGroups) {
+        for (int c0 = grp; c0 < nc; c0 += U * GROUPS) {
             float2 x[U];
             float4 y[U];
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const int64_t c = min(c0 + k * kJoinGroups, nc - 1);
+                const int64_t c = min(c0 + k * GROUPS, nc - 1);
                 x[k] = ml[c * step];
                 y[k] = *reinterpret_cast<const float4 *>(src + c * step * a.hd);
             }
@@ -54,15 +55,15 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs
             l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f, m = mn;
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                if (c0 + k * kJoinGroups >= nc || x[k].x == -INFINITY) continue;
+                if (c0 + k * GROUPS >= nc || x[k].x == -INFINITY) continue;
                 const float w = __builtin_amdgcn_exp2f((x[k].x - m) * kLog2e);
                 l += x[k].y * w;
                 o.x += y[k].x * w, o.y += y[k].y * w, o.z += y[k].z * w, o.w += y[k].w * w;
             }
         }
     };
-    if (nc <= kJoinGroups) take(std::integral_constant<int, 1>{});
-    else if (nc <= 4 * kJoinGroups) take(std::integral_constant<int, 4>{});
+    if (nc <= GROUPS) take(std::integral_constant<int, 1>{});
+    else if (nc <= 4 * GROUPS) take(std::integral_constant<int, 4>{});
     else take(std::integral_constant<int, 8>{});
     lds_o[grp][l16] = o;
     if (l16 == 0) lds_ml[grp] = float2{m, l};
@@ -70,10 +71,10 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs
     if (tid >= kJoinLanes || d >= a.hd) return;
     m = lds_ml[0].x;
 #pragma unroll
-    for (int g = 1; g < kJoinGroups; ++g) m = fmaxf(m, lds_ml[g].x);
+    for (int g = 1; g < GROUPS; ++g) m = fmaxf(m, lds_ml[g].x);
     l = 0.0f, o = float4{0, 0, 0, 0};
 #pragma unroll
-    for (int g = 0; g < kJoinGroups; ++g) {
+    for (int g = 0; g < GROUPS; ++g) {
         const float2 x = lds_ml[g];
         const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x.x - m) * kLog2e);
         const float4 y = lds_o[g][l16];
@@ -90,21 +91,34 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const JoinArgs
     if (a.lse && d == 0) a.lse[at] = some ? m + logf(l) : -INFINITY;
 }
 
-// How a call is cut: column tiles a workgroup takes, groups of them, and positions a chunk. The chunk is the longest of
-// 128 .. 512 that still gives every CU two workgroups over max_len: a short cache is cut fine (its time is latency), and
-// a chunk of 512 writes and reads back a few per cent of the bytes it reads.
+// How a call is cut: column tiles a workgroup takes, groups of them, and positions a chunk.
 struct AttnPlan {
-    int ct, col_groups, chunk, n_chunks;
+    int ct, col_groups, chunk, n_chunks, inner_heads;
 };
 static AttnPlan attn_plan(const gv_paged_kv &kv, const gv_paged_batch &b, int n_heads) {
     AttnPlan p;
     const int cols = b.max_rows * (n_heads / kv.n_kv_heads);
-    p.ct = 1;
+    p.ct = cols <= 16 ? 1 : kWideTiles;
     p.col_groups = (cols + 16 * p.ct - 1) / (16 * p.ct);
+    const bool wide = p.ct > 1 && kv.head_dim > 64;
     const int64_t items = static_cast<int64_t>(b.n_seqs) * kv.n_kv_heads * p.col_groups;
-    p.chunk = 512;
-    while (p.chunk > 128 && items * ((b.max_len + p.chunk - 1) / p.chunk) < 512) p.chunk /= 2;
+    if (wide) {
+        // Two workgroups a CU are there at once: the rounds of 64 positions that give each of the 512 the same number, the
+        // lengths of several sequences taken as three fifths of the longest. A workgroup that waits for another's end costs a
+        // whole one's time. Measured, chunks of 256 / 320 / 384 / 512: 32 sequences of up to 4,096 positions and 5 rows (16 heads
+        // of 256, fp16) 43 / 38 / 40 / 48 us; one of 32,001 positions and 17 rows (int8) 60 / 66 / 47 / 58.
+        const int64_t rounds = items * ((b.max_len + 63) / 64) * (b.n_seqs > 1 ? 3 : 5) / 5;
+        const int64_t each = (rounds + 511) / 512;
+        p.chunk = each <= 16 ? static_cast<int>(std::max<int64_t>(2, each)) * 64 : 512;
+    } else {
+        // The longest of 128 .. 512 that still gives every CU two workgroups over max_len: a short cache is cut fine (its time
+        // is latency), and a chunk of 512 writes and reads back a few per cent of the bytes it reads.
+        p.chunk = 512;
+        while (p.chunk > 128 && items * ((b.max_len + p.chunk - 1) / p.chunk) < 512) p.chunk /= 2;
+    }
     p.n_chunks = (b.max_len + p.chunk - 1) / p.chunk;
+    // (heads inside positions: a head's row of a position shares its cache lines with the next head's)
+    p.inner_heads = kv.head_stride < kv.pos_stride && static_cast<int64_t>(b.n_seqs) * p.n_chunks >= 64 ? kv.n_kv_heads : 1;
     return p;
 }
 static size_t attn_ws_bytes(const AttnPlan &p, const gv_paged_kv &kv, const gv_paged_batch &b, int n_heads) {
@@ -148,8 +162,8 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
     const size_t need = attn_ws_bytes(p, *kv, *batch, r->n_heads);
     GV_CHECK_ARG(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need),
                  "a 16-byte aligned workspace of gv_paged_attention_workspace_bytes");
-    const int64_t units = static_cast<int64_t>(batch->n_seqs) * kv->n_kv_heads * p.n_chunks;
-    const int64_t grid = (units + 7) / 8 * 8 * p.col_groups;
+    const int64_t units = static_cast<int64_t>(batch->n_seqs) * (kv->n_kv_heads / p.inner_heads) * p.n_chunks;
+    const int64_t grid = (units + 7) / 8 * 8 * p.col_groups * p.inner_heads;
     GV_CHECK_ARG(grid < int64_t{1} << 31, "too many sequences, heads and positions for one call");
     if (ensure_init() != 0) return -1;
     OnDevice dev;
@@ -163,7 +177,8 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
     a.ml = need ? a.parts + static_cast<size_t>(p.n_chunks) * batch->n_rows * r->n_heads * kv->head_dim : nullptr;
     a.q_row = r->q_row, a.out_row = r->out_row;
     a.nh = r->n_heads, a.group = r->n_heads / kv->n_kv_heads, a.type = r->type;
-    a.chunk = p.chunk, a.n_chunks = p.n_chunks, a.col_groups = p.col_groups;
+    a.group_inv = 1.0f / static_cast<float>(a.group);
+    a.chunk = p.chunk, a.n_chunks = p.n_chunks, a.col_groups = p.col_groups, a.inner_heads = p.inner_heads;
     a.scale = r->scale, a.faults = faults;
     const unsigned g = static_cast<unsigned>(grid);
     const int rc = kv->type == GV_F16    ? launch_attn_f16(a, p.ct, g, stream())
@@ -173,8 +188,11 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
     JoinArgs j{};
     j.b = a.b, j.parts = a.parts, j.ml = a.ml, j.out = a.out, j.lse = a.lse, j.out_row = a.out_row;
     j.nh = a.nh, j.hd = kv->head_dim, j.type = a.type, j.chunk = p.chunk;
-    hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>(batch->n_rows), static_cast<unsigned>(r->n_heads),
-                       static_cast<unsigned>((kv->head_dim + kJoinDims - 1) / kJoinDims)), dim3(kJoinThreads), 0, stream(), j);
+    // (few chunks: a wave a workgroup. 109 rows of 16 heads of 256 with up to 13 chunks 5.9 us where four waves take 10.6)
+    const dim3 grid_j(static_cast<unsigned>(batch->n_rows), static_cast<unsigned>(r->n_heads),
+                      static_cast<unsigned>((kv->head_dim + kJoinDims - 1) / kJoinDims));
+    if (p.n_chunks <= 16) hipLaunchKernelGGL(paged_join_kernel<4>, grid_j, dim3(4 * kJoinLanes), 0, stream(), j);
+    else hipLaunchKernelGGL(paged_join_kernel<16>, grid_j, dim3(16 * kJoinLanes), 0, stream(), j);
     GV_CHECK_HIP(hipGetLastError());
     return 0;
 }

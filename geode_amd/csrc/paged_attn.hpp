@@ -45,9 +45,11 @@ struct AttnArgs {
     float *parts, *ml;   // [chunk][row][head][hd] sums, [chunk][row][head][2] (maximum, sum of weights)
     int64_t q_row, out_row;
     int nh, group;       // query heads, and those of a KV head
+    float group_inv;     // 1 / group
     int type;            // of q and out
     int chunk, n_chunks; // positions a workgroup takes; chunks of max_len
     int col_groups;      // groups of CT x 16 columns that max_rows x group take
+    int inner_heads;     // KV heads whose workgroups follow each other: 1 or all of them
     float scale;
     int *faults;
 };
@@ -56,25 +58,19 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kAttnThreads = 256, kAttnWaves = 4, kAttnStep = 32;
 constexpr int kAttnMaxRows = 32;
 
-// Many columns of long rows: the sums of three column tiles x 256 dims would take 192 registers of a wave. Two waves then
-// share a step's positions and take half the dims of O^T each (both make the scores: the second's keys come from the
-// caches, and the matrix cores have the time).
-template <int NT, int CT>
-constexpr int attn_dim_split() {
-    return NT == 16 && CT > 1 ? 2 : 1;
-}
 // a kernel's LDS: the queries' operands, then (in the same place) the waves' sums of one column tile
 template <int NT, int CT, int QP>
 constexpr int attn_lds() {
     constexpr int q = CT * QP * (NT / 2) * 64 * 16;
-    constexpr int o = kAttnWaves / attn_dim_split<NT, CT>() * 16 * (NT * 16 + 4) * 4;
+    constexpr int o = kAttnWaves * 16 * (NT * 16 + 4) * 4;
     return q > o ? q : o;
 }
 
 // waves a SIMD a kernel's registers leave room for (asked of the compiler: more, and it spills)
-template <int KV, int NT, bool EX, int CT>
+template <int KV, int NT, bool EX, int CT, bool COUNTED>
 constexpr int attn_waves() {
-    if (CT > 1) return NT == 4 ? 2 : 1;
+    if (CT > 1) return COUNTED ? 1 : 2;
+    if (COUNTED) return NT == 4 ? 3 : NT == 8 ? 2 : 1;   // (the loop over the units takes a few more)
     return NT == 4 ? (KV == GV_I8 && !EX ? 3 : 4) : NT == 8 ? 3 : EX ? 2 : 1;
 }
 
@@ -100,27 +96,27 @@ __device__ inline float rows_sum(float v) {
     return a + b;
 }
 
-// N parts of 8 floats in the operand's type: each part the leading bits of what the parts before left (truncated, so
-// that the rest is exact)
-template <bool BF, int N>
-__device__ inline void split8(const float (&x)[8], au4 (&part)[N]) {
-    float r[8];
+// N parts of K floats in the operand's type, two to a word: each part the leading bits of what the parts before left
+// (truncated, so that the rest is exact)
+template <bool BF, int N, int K, typename Part>
+__device__ inline void split_parts(const float (&x)[K], Part &&put) {
+    float r[K];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = x[j];
+    for (int j = 0; j < K; ++j) r[j] = x[j];
 #pragma unroll
     for (int p = 0; p < N; ++p) {
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
+        for (int j = 0; j < K; j += 2) {
             if constexpr (BF) {
                 const uint32_t a = __builtin_bit_cast(uint32_t, r[j]), b = __builtin_bit_cast(uint32_t, r[j + 1]);
-                part[p][j / 2] = perm(b, a, 0x07060302u);
+                put(p, j / 2, perm(b, a, 0x07060302u));
                 if (p + 1 < N) {
                     r[j] -= __builtin_bit_cast(float, a & 0xFFFF0000u);
                     r[j + 1] -= __builtin_bit_cast(float, b & 0xFFFF0000u);
                 }
             } else {
                 const auto h = __builtin_amdgcn_cvt_pkrtz(r[j], r[j + 1]);
-                part[p][j / 2] = __builtin_bit_cast(uint32_t, h);
+                put(p, j / 2, __builtin_bit_cast(uint32_t, h));
                 if (p + 1 < N) {
                     r[j] -= static_cast<float>(h[0]);
                     r[j + 1] -= static_cast<float>(h[1]);
@@ -128,6 +124,14 @@ __device__ inline void split8(const float (&x)[8], au4 (&part)[N]) {
             }
         }
     }
+}
+template <bool BF, int N>
+__device__ inline void split8(const float (&x)[8], au4 (&part)[N]) {
+    split_parts<BF, N>(x, [&](int p, int j, uint32_t w) { part[p][j] = w; });
+}
+template <bool BF, int N>
+__device__ inline void split4(const float (&x)[4], uint2 (&part)[N]) {
+    split_parts<BF, N>(x, [&](int p, int j, uint32_t w) { (j ? part[p].y : part[p].x) = w; });
 }
 
 template <bool BF>
@@ -161,68 +165,213 @@ __device__ inline void load8(const char *p, int type, float (&x)[8]) {
     }
 }
 
+// ---------------------------------------------------------------- what both kernels begin with
+// A workgroup's unit: a chunk of a sequence's positions, a KV head, CT column tiles.
+struct AttnUnit {
+    Seq s;
+    int seq, head, chunk, p0, p1, ctx, nq, q0;   // positions [p0, p1) of len; ctx: those before its own rows; columns, first
+};
+// The index-th unit (false: there is none, or nothing in it to do). Column groups of a (sequence, chunk, KV head) follow
+// each other on one XCD (workgroups go round the eight), where the second finds the first's keys and values in the L2; so do the
+// KV heads where their rows share cache lines (inner_heads). The units are those of max_len, a chunk of every sequence after
+// the other, and the ones past a sequence's end are empty; or (COUNTED) every wave counts the chunks that the lengths
+// make, 64 sequences at a time, and takes the index-th of those.
+template <int CT, bool COUNTED>
+__device__ inline int attn_unit(const AttnArgs &a, unsigned index, AttnUnit &u) {   // 1: a unit, 0: an empty one, -1: past the last
+    const unsigned xcd = index & 7, idx = index >> 3, groups = static_cast<unsigned>(a.col_groups);
+    const unsigned inner = groups * static_cast<unsigned>(a.inner_heads), in = idx % inner;
+    const unsigned cg = in % groups, outer_heads = static_cast<unsigned>(a.kv.nkv / a.inner_heads);
+    unsigned unit = idx / inner * 8 + xcd, outer;
+    const int lane = threadIdx.x & 63;
+    if constexpr (COUNTED) {
+        int base = 0;
+        for (;; base += 64) {
+            if (base >= a.b.n_seqs) return -1;
+            const int i = min(base + lane, a.b.n_seqs - 1);
+            const int first = a.b.row_start[i], last = a.b.row_start[i + 1], len = a.b.lens[i];
+            const Seq s = make_seq(a.b, first, last, len);
+            const bool mine = base + lane < a.b.n_seqs;
+            if (mine && !s.fits) queue_fault(a.faults, kFaultRows);
+            const int n = mine && s.fits && s.rows > 0 ? (s.len + a.chunk - 1) / a.chunk * static_cast<int>(outer_heads) : 0;
+            const int incl = wave_incl_scan(n);
+            const unsigned all = static_cast<unsigned>(__builtin_amdgcn_readlane(incl, 63));
+            if (unit < all) {
+                const int at = __popcll(__ballot(static_cast<unsigned>(incl) <= unit));
+                u.seq = base + at;
+                u.s = make_seq(a.b, __builtin_amdgcn_readlane(first, at), __builtin_amdgcn_readlane(last, at), __builtin_amdgcn_readlane(len, at));
+                unit -= static_cast<unsigned>(__builtin_amdgcn_readlane(incl - n, at));
+                break;
+            }
+            unit -= all;
+        }
+        u.chunk = static_cast<int>(unit / outer_heads), outer = unit % outer_heads;
+    } else {
+        const unsigned items = static_cast<unsigned>(a.b.n_seqs) * outer_heads;
+        u.chunk = static_cast<int>(unit / items);
+        if (u.chunk >= a.n_chunks) return -1;
+        // (a chunk's items start three further on than the chunk before's: else each XCD would have the same sequences' chunks
+        // all along, and the XCD of the longest ones would end last)
+        const unsigned item = (unit % items + 3u * static_cast<unsigned>(u.chunk)) % items;
+        u.seq = static_cast<int>(item / outer_heads), outer = item % outer_heads;
+        u.s = seq_load(a.b, u.seq);
+        if (!u.s.fits) {
+            if (threadIdx.x == 0) queue_fault(a.faults, kFaultRows);
+            return 0;
+        }
+    }
+    u.head = static_cast<int>(outer) * a.inner_heads + static_cast<int>(in / groups);
+    u.p0 = u.chunk * a.chunk;
+    u.nq = u.s.rows * a.group, u.q0 = static_cast<int>(cg) * CT * 16;
+    u.ctx = u.s.len - u.s.rows, u.p1 = min(u.p0 + a.chunk, u.s.len);
+    return u.q0 < u.nq && u.p0 < u.s.len;
+}
+
+// A tile of 16 positions a lane: where its keys and values lie. One that is not wanted, lies past the chunk or names a page
+// outside the pool reads the pool's first page (lost: the last was met; usable: the lanes' tiles that count).
+struct AttnTiles {
+    int64_t off, scale_off;   // elements
+    uint64_t usable;
+    bool lost;
+};
+__device__ inline AttnTiles attn_tiles(const AttnArgs &a, const AttnUnit &u, int tile, bool wanted) {
+    const int entry = min(tile, a.b.max_len - 1) / a.kv.page;   // (within the table's row whatever the length)
+    const int page = a.b.pages[u.seq * a.b.ld_pages + entry];
+    const bool own = wanted && tile < u.p1, good = page >= 0 && page < a.kv.n_pages;
+    if (own && !good) queue_fault(a.faults, kFaultPage);
+    AttnTiles t;
+    t.lost = __any(own && !good);
+    t.usable = __ballot(own && good);
+    const int64_t pg = own && good ? page : 0;
+    const int slot = tile % a.kv.page;
+    t.off = pg * a.kv.page_stride + u.head * a.kv.head_stride + slot * a.kv.pos_stride;
+    t.scale_off = (pg * a.kv.nkv + u.head) * a.kv.page + slot;
+    return t;
+}
+__device__ inline int64_t lane64(int64_t v, int l) {   // lane l's value, uniform
+    const uint64_t u = static_cast<uint64_t>(v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u)), l);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u >> 32)), l);
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Loads from a uniform place plus a lane's 32-bit byte offset and a uniform one: buffer instructions, whose addresses take
+// no vector registers (a 64-bit address a lane and load took up to 40).
+typedef uint32_t au2 __attribute__((ext_vector_type(2)));
+__device__ inline __amdgpu_buffer_rsrc_t place(const void *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), static_cast<short>(0), 0x7FFFFFFF, 0x00020000);
+}
+__device__ inline au4 load16(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
+    return __builtin_amdgcn_raw_buffer_load_b128(r, lane_off, off, 0);
+}
+__device__ inline au2 load8b(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
+    return __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, off, 0);
+}
+__device__ inline uint32_t load4b(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
+    return __builtin_amdgcn_raw_buffer_load_b32(r, lane_off, off, 0);
+}
+__device__ inline float4 load4f(const float *p, uint32_t lane_off) { return __builtin_bit_cast(float4, load16(place(p), lane_off, 0)); }
+
+// x / group of a column x < 32 group (group at most 4,096): the quotient's distance to a whole number, at least 0.5 / group,
+// is far above the error of 32 x 2^-22
+__device__ inline int row_of(const AttnArgs &a, int x) { return static_cast<int>((static_cast<float>(x) + 0.5f) * a.group_inv); }
+
+// The columns' powers of two (fp16 products of other types' queries): a column's largest value to 2^10 .. 2^11 (0 and not
+// finite: left). A lane's column is 16 ct + lane % 16.
+struct QueryScale {
+    const float *amax;
+    bool scaled;
+    __device__ int exponent(int ct) const {
+        const int e = static_cast<int>(__float_as_uint(amax[ct * 16 + (threadIdx.x & 15)]) >> 23);
+        return scaled && e > 0 && e < 255 ? min(max(137 - e, -126), 126) : 0;
+    }
+    __device__ float undo(int ct) const { return __uint_as_float(static_cast<uint32_t>(127 - exponent(ct)) << 23); }
+};
+// The queries' operands to LDS in the order the products take them, [column tile][part][chunk][lane], by the whole
+// workgroup; ends with a barrier.
+template <bool BF, bool I8, int QP, int NCH, bool EX, int CT>
+__device__ inline QueryScale stage_queries(const AttnArgs &a, const AttnUnit &u, au4 *lds_q, float *lds_amax) {
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, i16 = lane & 15, g4 = lane >> 4;
+    const QueryScale qs{lds_amax, !BF && a.type != GV_F16};
+    const int qes = a.type == GV_F32 ? 4 : 2;
+    if (qs.scaled) {
+        for (int i = tid; i < CT * 16; i += kAttnThreads) lds_amax[i] = 0.0f;
+        __syncthreads();
+    }
+    constexpr int QU = (CT * NCH * 64 + kAttnThreads - 1) / kAttnThreads;
+    float qv[QU][8];
+#pragma unroll
+    for (int k = 0; k < QU; ++k) {
+        const int w = k * kAttnThreads + tid, c = w / 64 % NCH, ct = w / 64 / NCH;
+        const int x = u.q0 + ct * 16 + i16;
+        const int d = I8 ? (c >> 1) * 64 + g4 * 16 + (c & 1) * 8 : c * 32 + g4 * 8;
+        const bool in = ct < CT && x < u.nq && (EX || d < a.kv.hd);
+        const int xc = in ? x : 0, r = row_of(a, xc);
+        load8(a.q + ((u.s.first + r) * a.q_row + static_cast<int64_t>(u.head * a.group + xc - r * a.group) * a.kv.hd + (in ? d : 0)) * qes,
+              a.type, qv[k]);
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            qv[k][j] = in ? qv[k][j] : 0.0f;
+            m = fmaxf(m, fabsf(qv[k][j]));
+        }
+        if (qs.scaled) {   // (positive floats order as their bits)
+            m = rows_max(m);
+            if (lane < 16 && ct < CT) atomicMax(reinterpret_cast<unsigned *>(lds_amax) + ct * 16 + i16, __float_as_uint(m));
+        }
+    }
+    if (qs.scaled) __syncthreads();
+#pragma unroll
+    for (int k = 0; k < QU; ++k) {
+        const int w = k * kAttnThreads + tid, c = w / 64 % NCH, ct = w / 64 / NCH;
+        if (ct >= CT) continue;
+        if (qs.scaled) {
+            const float f = __uint_as_float(static_cast<uint32_t>(127 + qs.exponent(ct)) << 23);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) qv[k][j] *= f;
+        }
+        au4 part[QP];
+        split8<BF, QP>(qv[k], part);
+#pragma unroll
+        for (int p = 0; p < QP; ++p) lds_q[((ct * QP + p) * NCH + c) * 64 + lane] = part[p];
+    }
+    __syncthreads();
+    return qs;
+}
+// which of its sequence's rows column x sees
+__device__ inline uint32_t seen_rows(const AttnArgs &a, const AttnUnit &u, int x) {
+    const int r = row_of(a, x);
+    return x >= u.nq ? 0u : a.visible ? a.visible[u.s.first + r] : 0xFFFFFFFFu >> (31 - r);
+}
+
+// ---------------------------------------------------------------- few columns
 // KV: the cache's type. QP, PP: the parts of the queries and of the weights. NT: dim tiles of 16 (head_dim at most
 // 16 NT; EX: exactly). CT: column tiles of 16 queries a workgroup takes.
 template <int KV, int QP, int PP, int NT, bool EX, int CT>
-__global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void paged_attn_kernel(const AttnArgs a) {
+__device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
     constexpr bool BF = KV == GV_BF16, I8 = KV == GV_I8;
     constexpr int ES = I8 ? 1 : 2;         // bytes a cached element
     constexpr int NCH = NT / 2;            // 32-dim chunks of S^T's products
     constexpr int KL = I8 ? NCH / 2 : NCH; // 16-byte loads a lane a K tile
-    constexpr int DS = attn_dim_split<NT, CT>(), NV = NT / DS, PW = kAttnWaves / DS;   // (see there)
-    constexpr int VW = NV * ES / 4;        // words a lane a V row
+    constexpr int VW = NT * ES / 4;        // words a lane a V row
     extern __shared__ au4 lds_q[];         // [CT][QP][NCH][64]
     __shared__ float lds_amax[CT * 16];
-    __shared__ float lds_m[PW][CT * 16], lds_l[PW][CT * 16], lds_e[PW][CT * 16];
-    touch_args(a);
+    __shared__ float lds_m[kAttnWaves][CT * 16], lds_l[kAttnWaves][CT * 16], lds_e[kAttnWaves][CT * 16];
     const int lane = threadIdx.x & 63, i16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));   // (uniform: its branches are)
-    const int pw = wave / DS, half = wave % DS;   // whose positions, which dims
 
-    // which unit: column groups of a (chunk, sequence, KV head) follow each other on one XCD (workgroups go round the
-    // eight), where the second finds the first's keys and values in the L2
-    const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
-    const int cg = idx % a.col_groups;
-    const int64_t unit = static_cast<int64_t>(idx / a.col_groups) * 8 + xcd;
-    const int items = a.b.n_seqs * a.kv.nkv;
-    const int chunk = static_cast<int>(unit / items), item = static_cast<int>(unit % items);
-    if (chunk >= a.n_chunks) return;
-    const int seq = item / a.kv.nkv, head = item % a.kv.nkv;
-    const int p0 = chunk * a.chunk;
-
-    // every load that needs only the sequence at once: its rows and length, and the pages of this wave's tiles (lane t:
-    // step t / 2, tile t % 2; entries past the table's last are not read)
-    const int tile = p0 + kAttnStep * (pw + PW * (lane >> 1)) + 16 * (lane & 1);
-    const int64_t entry = tile / a.kv.page;
-    const int page = a.b.pages[seq * a.b.ld_pages + min(entry, static_cast<int64_t>(a.b.max_len - 1) / a.kv.page)];
-    const Seq s = seq_load(a.b, seq);
-    if (!s.fits) {
-        if (threadIdx.x == 0) queue_fault(a.faults, kFaultRows);
-        return;
-    }
-    const int nq = s.rows * a.group, q0 = cg * CT * 16;
-    if (q0 >= nq || p0 >= s.len) return;
-    const int ctx = s.len - s.rows, p1 = min(p0 + a.chunk, s.len);
-    const bool own_tile = tile < p1 && (lane >> 1) * PW * kAttnStep < a.chunk;
-    const bool good = page >= 0 && page < a.kv.n_pages;
-    if (own_tile && !good) queue_fault(a.faults, kFaultPage);
-    const bool lost = __any(own_tile && !good);   // (a page outside the pool: its positions read as not seen)
-    const uint64_t usable = __ballot(own_tile && good);
-    const int slot = tile % a.kv.page;
-    const int pg = own_tile && good ? page : 0;
-    const int64_t toff = pg * a.kv.page_stride + head * a.kv.head_stride + slot * a.kv.pos_stride;   // elements
-    const int64_t soff = (static_cast<int64_t>(pg) * a.kv.nkv + head) * a.kv.page + slot;
+    const Seq &s = u.s;
+    const int p0 = u.p0, p1 = u.p1, ctx = u.ctx, nq = u.nq, q0 = u.q0, head = u.head;
+    // the pages of this wave's tiles (lane t: step t / 2, tile t % 2)
+    const int tile = p0 + kAttnStep * (wave + kAttnWaves * (lane >> 1)) + 16 * (lane & 1);
+    const AttnTiles at = attn_tiles(a, u, tile, (lane >> 1) * kAttnWaves * kAttnStep < a.chunk);
+    const int64_t toff = at.off, soff = at.scale_off;
+    const uint64_t usable = at.usable;
+    const bool lost = at.lost;
 
     const uint32_t klane = (static_cast<uint32_t>(i16) * static_cast<uint32_t>(a.kv.pos_stride) + g4 * (I8 ? 16 : 8)) * ES;
-    const int vdim = half * NV * 16 + i16 * NV;   // the lane's first dim of the values
-    const uint32_t vlane = (static_cast<uint32_t>(4 * g4) * static_cast<uint32_t>(a.kv.pos_stride) + vdim) * ES;
+    const uint32_t vlane = (static_cast<uint32_t>(4 * g4) * static_cast<uint32_t>(a.kv.pos_stride) + i16 * NT) * ES;
     const uint32_t vrow = static_cast<uint32_t>(a.kv.pos_stride) * ES;
-    const auto lane64 = [](int64_t v, int l) {
-        const uint64_t u = static_cast<uint64_t>(v);
-        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u)), l);
-        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(u >> 32)), l);
-        return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-    };
 
     // ---- one step's operands: keys (with their scales) and values; a tile that is not used reads the pool's first page
     au4 kf[2][KL];
@@ -231,20 +380,20 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
     const auto load_k = [&](int st) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const char *kb = a.kv.k + lane64(toff, 2 * st + h) * ES;
+            const auto kb = place(a.kv.k + lane64(toff, 2 * st + h) * ES);
 #pragma unroll
             for (int c = 0; c < KL; ++c) {
                 constexpr uint32_t per = I8 ? 64 : 32 * ES;   // bytes between a lane's loads
                 if constexpr (EX) {
-                    kf[h][c] = *reinterpret_cast<const au4 *>(kb + klane + c * per);
+                    kf[h][c] = load16(kb, klane + c * per, 0);
                 } else {
                     const int d = I8 ? c * 64 + g4 * 16 : c * 32 + g4 * 8;
-                    const au4 w = *reinterpret_cast<const au4 *>(kb + (d < a.kv.hd ? klane + c * per : 0));
+                    const au4 w = load16(kb, d < a.kv.hd ? klane + c * per : 0, 0);
                     kf[h][c] = d < a.kv.hd ? w : au4{0, 0, 0, 0};
                 }
             }
             if constexpr (I8) {
-                const float4 x = *reinterpret_cast<const float4 *>(a.kv.ks + lane64(soff, 2 * st + h) + 4 * g4);
+                const float4 x = load4f(a.kv.ks + lane64(soff, 2 * st + h), 16 * g4);
                 ksc[h][0] = x.x, ksc[h][1] = x.y, ksc[h][2] = x.z, ksc[h][3] = x.w;
             }
         }
@@ -252,34 +401,33 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
     const auto load_v = [&](int st) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const char *vb = a.kv.v + lane64(toff, 2 * st + h) * ES;
-            const bool in = EX || vdim < a.kv.hd;
+            const auto vb = place(a.kv.v + lane64(toff, 2 * st + h) * ES);
+            const uint32_t lo = EX || i16 * NT < a.kv.hd ? vlane : 0;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const char *src = vb + (in ? vlane + r * vrow : 0);
                 uint32_t(&w)[VW] = vr[4 * h + r];
                 if constexpr (VW >= 4) {
 #pragma unroll
                     for (int k = 0; k < VW / 4; ++k) {
-                        const au4 x = *reinterpret_cast<const au4 *>(src + 16 * k);
+                        const au4 x = load16(vb, lo + 16 * k, r * vrow);
                         w[4 * k] = x[0], w[4 * k + 1] = x[1], w[4 * k + 2] = x[2], w[4 * k + 3] = x[3];
                     }
                 } else if constexpr (VW == 2) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
-                    w[0] = x.x, w[1] = x.y;
+                    const au2 x = load8b(vb, lo, r * vrow);
+                    w[0] = x[0], w[1] = x[1];
                 } else {
-                    w[0] = *reinterpret_cast<const uint32_t *>(src);
+                    w[0] = load4b(vb, lo, r * vrow);
                 }
             }
             if constexpr (I8) {
-                const float4 y = *reinterpret_cast<const float4 *>(a.kv.vs + lane64(soff, 2 * st + h) + 4 * g4);
+                const float4 y = load4f(a.kv.vs + lane64(soff, 2 * st + h), 16 * g4);
                 vsc[h][0] = y.x, vsc[h][1] = y.y, vsc[h][2] = y.z, vsc[h][3] = y.w;
             }
         }
     };
 
-    const int mine = p1 - p0 - kAttnStep * pw, open = ctx - p0 - kAttnStep * (pw + 1);
-    constexpr int kRound = kAttnStep * PW;
+    const int mine = p1 - p0 - kAttnStep * wave, open = ctx - p0 - kAttnStep * (wave + 1);
+    constexpr int kRound = kAttnStep * kAttnWaves;
     const int steps = mine > 0 ? (mine + kRound - 1) / kRound : 0;
     const int free_steps = lost || open < 0 ? 0 : min(steps, open / kRound + 1);
     if (steps > 0) {   // (the first step's keys and values on their way while the queries are made ready)
@@ -287,74 +435,28 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
         load_v(0);
     }
 
-    // the queries' operands, in the order the products take them: [column tile][part][chunk][lane]
-    for (int i = threadIdx.x; i < CT * 16; i += kAttnThreads) lds_amax[i] = 0.0f;
-    const bool scaled = !BF && a.type != GV_F16;
+    const QueryScale qs = stage_queries<BF, I8, QP, NCH, EX, CT>(a, u, lds_q, lds_amax);
     const int qes = a.type == GV_F32 ? 4 : 2;
-    if (scaled) __syncthreads();
-    constexpr int QU = CT * NCH * 64 / kAttnThreads > 0 ? (CT * NCH * 64 + kAttnThreads - 1) / kAttnThreads : 1;
-    float qv[QU][8];
-#pragma unroll
-    for (int u = 0; u < QU; ++u) {
-        const int w = u * kAttnThreads + threadIdx.x, c = w / 64 % NCH, ct = w / 64 / NCH;
-        const int x = q0 + ct * 16 + i16;
-        const int d = I8 ? (c >> 1) * 64 + g4 * 16 + (c & 1) * 8 : c * 32 + g4 * 8;
-        const bool in = ct < CT && x < nq && (EX || d < a.kv.hd);
-        const int xc = in ? x : 0;
-        load8(a.q + ((s.first + xc / a.group) * a.q_row + static_cast<int64_t>(head * a.group + xc % a.group) * a.kv.hd + (in ? d : 0)) * qes,
-              a.type, qv[u]);
-        float m = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            qv[u][j] = in ? qv[u][j] : 0.0f;
-            m = fmaxf(m, fabsf(qv[u][j]));
-        }
-        // (positive floats order as their bits; an infinity is caught below)
-        if (scaled && in) atomicMax(reinterpret_cast<unsigned *>(lds_amax) + ct * 16 + i16, __float_as_uint(m));
-    }
-    if (scaled) __syncthreads();
-    // a column's power of two: its largest value to 2^10 .. 2^11 (0 and not finite: left)
-    const auto exponent = [&](int ct) {
-        const uint32_t b = __float_as_uint(lds_amax[ct * 16 + i16]);
-        const int e = static_cast<int>(b >> 23);
-        return scaled && e > 0 && e < 255 ? min(max(137 - e, -126), 126) : 0;
-    };
-#pragma unroll
-    for (int u = 0; u < QU; ++u) {
-        const int w = u * kAttnThreads + threadIdx.x, c = w / 64 % NCH, ct = w / 64 / NCH;
-        if (ct >= CT) continue;
-        if (scaled) {
-            const float f = __uint_as_float(static_cast<uint32_t>(127 + exponent(ct)) << 23);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) qv[u][j] *= f;
-        }
-        au4 part[QP];
-        split8<BF, QP>(qv[u], part);
-#pragma unroll
-        for (int p = 0; p < QP; ++p) lds_q[((ct * QP + p) * NCH + c) * 64 + lane] = part[p];
-    }
-    __syncthreads();
 
     float sc[CT], m[CT], l[CT], ex[CT];   // a column's score factor, maximum, sum; int8: the power of two its weights have
     uint32_t bits[CT];                    // which of the sequence's rows it sees
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        sc[ct] = a.scale * __uint_as_float(static_cast<uint32_t>(127 - exponent(ct)) << 23) * (I8 ? kI8Unit : 1.0f);
+        sc[ct] = a.scale * qs.undo(ct) * (I8 ? kI8Unit : 1.0f);
         m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = 0.0f;
-        const int x = q0 + ct * 16 + i16, r = x / a.group;
-        bits[ct] = x >= nq ? 0u : a.visible ? a.visible[s.first + r] : 0xFFFFFFFFu >> (31 - r);
+        bits[ct] = seen_rows(a, u, q0 + ct * 16 + i16);
     }
-    af4 acc[CT][NV];
+    af4 acc[CT][NT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int n = 0; n < NV; ++n) acc[ct][n] = af4{0, 0, 0, 0};
+        for (int n = 0; n < NT; ++n) acc[ct][n] = af4{0, 0, 0, 0};
 
     // One step: the next step's keys are asked for once this one's are in the products, its values likewise. `tail`: a
     // step with positions that some query does not see (the sequence's own rows, its end, a lost page).
     const auto step = [&](auto tail_c, int st, bool more) {
         constexpr bool tail = decltype(tail_c)::value;
-        const int p = p0 + kAttnStep * (pw + PW * st);
+        const int p = p0 + kAttnStep * (wave + kAttnWaves * st);
         int ql = lane;   // (pinned: the queries are read from LDS in every step, not kept in registers)
         if constexpr (CT * NT * QP >= 16) asm volatile("" : "+v"(ql));
         // ---- scores
@@ -441,7 +543,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
                 l[ct] *= gone;
                 const float f = I8 && en > ex[ct] ? gone * (ex[ct] / en) : gone;
 #pragma unroll
-                for (int n = 0; n < NV; ++n) acc[ct][n] *= f;
+                for (int n = 0; n < NT; ++n) acc[ct][n] *= f;
                 m[ct] = mn, ex[ct] = en;
             }
             const float base = mn == -INFINITY ? 0.0f : mn;
@@ -479,7 +581,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
         };
         if constexpr (!tail || I8) {
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
+            for (int n = 0; n < NT; ++n) {
                 const au4 v = v_tile(n);
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
@@ -519,7 +621,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
 #pragma unroll
                 for (int k = 0; k < VW; ++k) asm volatile("" : "+v"(vr[r][k]));
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
+            for (int n = 0; n < NT; ++n) {
                 au4 v = v_tile(n);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] &= keep[k];
@@ -550,7 +652,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         l[ct] = rows_sum(l[ct]);
-        if (half == 0 && lane < 16) lds_m[pw][ct * 16 + lane] = m[ct], lds_l[pw][ct * 16 + lane] = l[ct], lds_e[pw][ct * 16 + lane] = ex[ct];
+        if (lane < 16) lds_m[wave][ct * 16 + lane] = m[ct], lds_l[wave][ct * 16 + lane] = l[ct], lds_e[wave][ct * 16 + lane] = ex[ct];
     }
     __syncthreads();
     const bool whole = s.len <= a.chunk;
@@ -560,34 +662,34 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
         const int col = ct * 16 + i16;
         float mt = lds_m[0][col], et = lds_e[0][col];
 #pragma unroll
-        for (int w = 1; w < PW; ++w) mt = fmaxf(mt, lds_m[w][col]), et = fmaxf(et, lds_e[w][col]);
+        for (int w = 1; w < kAttnWaves; ++w) mt = fmaxf(mt, lds_m[w][col]), et = fmaxf(et, lds_e[w][col]);
         float f = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mt) * kLog2e);
         if constexpr (I8) f = et > 0.0f ? f * (ex[ct] / et) : 0.0f;
-        float *o = lds_o + (pw * 16 + i16) * OLD + half * NV * 16;
+        float *o = lds_o + (wave * 16 + i16) * OLD;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int n = 0; n < NV; n += 4)
-                *reinterpret_cast<float4 *>(o + (4 * g4 + r) * NV + n) =
+            for (int n = 0; n < NT; n += 4)
+                *reinterpret_cast<float4 *>(o + (4 * g4 + r) * NT + n) =
                     float4{acc[ct][n][r] * f, acc[ct][n + 1][r] * f, acc[ct][n + 2][r] * f, acc[ct][n + 3][r] * f};
         __syncthreads();
-        for (int u = threadIdx.x; u < 16 * NT * 4; u += kAttnThreads) {
-            const int c = u / (NT * 4), d = u % (NT * 4) * 4;
+        for (int e = threadIdx.x; e < 16 * NT * 4; e += kAttnThreads) {
+            const int c = e / (NT * 4), d = e % (NT * 4) * 4;
             const int x = q0 + ct * 16 + c;
             if (x >= nq || (!EX && d >= a.kv.hd)) continue;
             float mm = lds_m[0][ct * 16 + c], ee = lds_e[0][ct * 16 + c];
 #pragma unroll
-            for (int w = 1; w < PW; ++w) mm = fmaxf(mm, lds_m[w][ct * 16 + c]), ee = fmaxf(ee, lds_e[w][ct * 16 + c]);
+            for (int w = 1; w < kAttnWaves; ++w) mm = fmaxf(mm, lds_m[w][ct * 16 + c]), ee = fmaxf(ee, lds_e[w][ct * 16 + c]);
             float ll = 0.0f;
             float4 v = float4{0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < PW; ++w) {
+            for (int w = 0; w < kAttnWaves; ++w) {
                 const float mw = lds_m[w][ct * 16 + c];
                 if (mw != -INFINITY) ll += lds_l[w][ct * 16 + c] * __builtin_amdgcn_exp2f((mw - mm) * kLog2e);
                 const float4 y = *reinterpret_cast<const float4 *>(lds_o + (w * 16 + c) * OLD + d);
                 v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
             }
-            const int row = s.first + x / a.group, hq = head * a.group + x % a.group;
+            const int r = row_of(a, x), row = s.first + r, hq = head * a.group + x - r * a.group;
             const float unit_v = BF ? 1.0f : I8 ? ee * (kI8Unit / 16384.0f) : 1.0f / 16384.0f;
             v.x *= unit_v, v.y *= unit_v, v.z *= unit_v, v.w *= unit_v;
             if (whole) {
@@ -599,43 +701,58 @@ __global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT>())) void 
                 else store4<GV_BF16>(dst, v);
                 if (a.lse && d == 0) a.lse[static_cast<int64_t>(row) * a.nh + hq] = ll > 0.0f || ll != ll ? mm + logf(ll) : -INFINITY;
             } else {
-                const int64_t at = (static_cast<int64_t>(chunk) * a.b.n_rows + row) * a.nh + hq;
-                store4<GV_F32>(reinterpret_cast<char *>(a.parts + at * a.kv.hd + d), v);
-                if (d == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = float2{mm, ll};
+                const int64_t to = (static_cast<int64_t>(u.chunk) * a.b.n_rows + row) * a.nh + hq;
+                store4<GV_F32>(reinterpret_cast<char *>(a.parts + to * a.kv.hd + d), v);
+                if (d == 0) *reinterpret_cast<float2 *>(a.ml + to * 2) = float2{mm, ll};
             }
         }
         __syncthreads();
     }
 }
 
+// COUNTED: a workgroup takes one unit after the other of those that the lengths make (attn_unit)
+template <int KV, int QP, int PP, int NT, bool EX, int CT, bool COUNTED>
+__global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT, COUNTED>())) void paged_attn_kernel(const AttnArgs a) {
+    touch_args(a);
+    AttnUnit u;
+    if constexpr (!COUNTED) {
+        if (attn_unit<CT, false>(a, blockIdx.x, u) > 0) attn_few_columns<KV, QP, PP, NT, EX, CT>(a, u);
+        return;
+    }
+    for (unsigned i = blockIdx.x;; i += gridDim.x) {
+        const int is = attn_unit<CT, true>(a, i, u);
+        if (is < 0) return;
+        if (is > 0) attn_few_columns<KV, QP, PP, NT, EX, CT>(a, u);
+        __syncthreads();
+    }
+}
+
+// the column tiles a workgroup takes where there is more than one
+constexpr int kWideTiles = 3;
 // the kernels of one cache type, by parts (16-bit or fp32 rows), dims and column tiles (paged_attn_<type>.hip)
 int launch_attn_f16(const AttnArgs &a, int ct, unsigned grid, hipStream_t st);
 int launch_attn_bf16(const AttnArgs &a, int ct, unsigned grid, hipStream_t st);
 int launch_attn_i8(const AttnArgs &a, int ct, unsigned grid, hipStream_t st);
 
-template <int KV, int QP, int PP, int NT, bool EX, int CT>
+template <int KV, int QP, int PP, int NT, bool EX, int CT, bool COUNTED>
 int launch_attn_one(const AttnArgs &a, unsigned grid, hipStream_t st) {
     constexpr int lds = attn_lds<NT, CT, QP>();
     static int granted = 0;
-    if (lds_grant(reinterpret_cast<const void *>(&paged_attn_kernel<KV, QP, PP, NT, EX, CT>), lds, granted) != 0) return -1;
-    hipLaunchKernelGGL((paged_attn_kernel<KV, QP, PP, NT, EX, CT>), dim3(grid), dim3(kAttnThreads), lds, st, a);
+    if (lds_grant(reinterpret_cast<const void *>(&paged_attn_kernel<KV, QP, PP, NT, EX, CT, COUNTED>), lds, granted) != 0) return -1;
+    hipLaunchKernelGGL((paged_attn_kernel<KV, QP, PP, NT, EX, CT, COUNTED>), dim3(grid), dim3(kAttnThreads), lds, st, a);
     GV_CHECK_HIP(hipGetLastError());
     return 0;
 }
-template <int KV, int QP, int PP, int NT, bool EX>
-int launch_attn_ct(const AttnArgs &a, int ct, unsigned grid, hipStream_t st) {
-    return ct == 1 ? launch_attn_one<KV, QP, PP, NT, EX, 1>(a, grid, st) : launch_attn_one<KV, QP, PP, NT, EX, 3>(a, grid, st);
+// The units by max_len, or COUNTED in as many workgroups as are there at once: where there are more than 32 units a CU. An
+// empty workgroup keeps its place for a microsecond, so that a batch with one long sequence spends its time on them: one
+// of 65,537 positions among thirty short ones (24 heads of 80, bf16; 16,000 units, most of them empty) 44 us by max_len,
+// 28 counted; 64 full sequences of 8,192 (8,192 units) 137 and 139. Each unit scans the lengths, so only up to
+// kCountSeqs sequences.
+constexpr int kCountUnits = 32 * 256, kCountSeqs = 256;
+template <int KV, int QP, int PP, int NT, bool EX, int CT>
+int launch_attn_few(const AttnArgs &a, unsigned grid, hipStream_t st) {
+    if (grid > kCountUnits && a.b.n_seqs <= kCountSeqs)
+        return launch_attn_one<KV, QP, PP, NT, EX, CT, true>(a, 256 * attn_waves<KV, NT, EX, CT, true>(), st);
+    return launch_attn_one<KV, QP, PP, NT, EX, CT, false>(a, grid, st);
 }
-template <int KV, int QP, int PP>
-int launch_attn_nt(const AttnArgs &a, int ct, unsigned grid, hipStream_t st) {
-    switch (a.kv.hd) {
-    case 64: return launch_attn_ct<KV, QP, PP, 4, true>(a, ct, grid, st);
-    case 128: return launch_attn_ct<KV, QP, PP, 8, true>(a, ct, grid, st);
-    case 256: return launch_attn_ct<KV, QP, PP, 16, true>(a, ct, grid, st);
-    }
-    return a.kv.hd < 64 ? launch_attn_ct<KV, QP, PP, 4, false>(a, ct, grid, st)
-           : a.kv.hd < 128 ? launch_attn_ct<KV, QP, PP, 8, false>(a, ct, grid, st)
-                           : launch_attn_ct<KV, QP, PP, 16, false>(a, ct, grid, st);
-}
-
 }  // namespace gv

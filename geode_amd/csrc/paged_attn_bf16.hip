@@ -1,5 +1,5 @@
 // paged_attn_bf16.hip - the paged attention's kernels over a bf16 cache.
-#include "paged_attn.hpp"
+#include "paged_attn_wide.hpp"
 
 namespace gv {
 

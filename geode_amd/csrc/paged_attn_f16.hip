@@ -1,5 +1,5 @@
 // paged_attn_f16.hip - the paged attention's kernels over an fp16 cache.
-#include "paged_attn.hpp"
+#include "paged_attn_wide.hpp"
 
 namespace gv {
 

@@ -1,5 +1,5 @@
 // paged_attn_i8.hip - the paged attention's kernels over an int8 cache.
-#include "paged_attn.hpp"
+#include "paged_attn_wide.hpp"
 
 namespace gv {
 

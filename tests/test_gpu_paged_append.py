@@ -115,6 +115,14 @@ def test_a_rows_sequence_is_found(gv, n_seqs):
          n_rows=int(rows.sum()) + 8, first_row=3)
 
 
+@pytest.mark.parametrize("cache,kind", [("f16", "f32"), ("i8", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("nh,nkv,hd,rope,interleaved", [(9, 3, 256, 64, False), (7, 5, 64, 64, False), (6, 1, 128, 96, True)])
+def test_prompts(gv, cache, kind, nh, nkv, hd, rope, interleaved):
+    """many rows: several rounds of heads a wave, four heads a lane group, the last of them not whole"""
+    _run(gv, 42, cache, kind, kind, [700, 800, 3000], [700, 811, 3000], page=64, nh=nh, nkv=nkv, hd=hd, rope=rope,
+         interleaved=interleaved)
+
+
 def test_tree_positions_and_far_angles(gv):
     """rotary positions apart from the places in the cache (a draft tree's depths), near the tables' end"""
     pos = np.array([8990, 8991, 8991, 8991, 8992, 8999], np.int32)

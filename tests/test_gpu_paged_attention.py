@@ -70,7 +70,7 @@ def test_chains(gv, cache, kind, rows):
 
 
 @pytest.mark.parametrize("cache,kind", [("f16", "f32"), ("bf16", "bf16"), ("i8", "f16")])
-@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("hd", [64, 128, 192, 256])
 def test_tree_and_rows_that_see_nothing(gv, cache, kind, hd):
     """a row's own bits alone decide what it sees of its sequence's rows: a tree, a row that does not see itself, and in a
     sequence without context rows that see nothing"""
@@ -82,12 +82,14 @@ def test_tree_and_rows_that_see_nothing(gv, cache, kind, hd):
 
 
 @pytest.mark.parametrize("cache,kind", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
-def test_values_a_row_does_not_see(gv, cache, kind):
-    """NaNs and infinities in later rows' keys and values reach the rows that see them and no others"""
-    f = Filled(12, cache, [6, 5], [70, 5], 16, 2, 64)
+@pytest.mark.parametrize("nh,hd", [(4, 64), (16, 64), (4, 128), (16, 128), (16, 96), (4, 256), (16, 256), (16, 192)])
+def test_values_a_row_does_not_see(gv, cache, kind, nh, hd):
+    """NaNs and infinities in later rows' keys and values reach the rows that see them and no others (few and many columns
+    a KV head)"""
+    f = Filled(12, cache, [6, 5], [70, 5], 16, 2, hd)
     clean = {n: f.host[n].copy() for n in ("k", "v")}
-    q = _queries(13, 11, 4, 64, kind)
-    scale = float(np.float32(0.125))
+    q = _queries(13, 11, nh, hd, kind)
+    scale = float(np.float32(hd ** -0.5))
     base, _ = gv.paged_attention(f.cache, f.batch, q, type_=TYPES[kind], scale=scale)
     for name, val in (("v", np.nan), ("v", np.inf), ("k", np.nan), ("v", -np.inf)):
         f.host[name] = clean[name].copy()
@@ -99,22 +101,54 @@ def test_values_a_row_does_not_see(gv, cache, kind):
         blind = np.array([0, 1, 2, 6, 7, 8])        # rows before it
         assert np.array_equal(got[blind], base[blind]), (name, val)
         sees = np.array([3, 4, 5, 9, 10])
-        assert np.array_equal(got[sees][:, :2], base[sees][:, :2])     # the other KV head's query heads
+        assert np.array_equal(got[sees][:, :nh // 2], base[sees][:, :nh // 2])     # the other KV head's query heads
         if name == "v":
-            others = np.arange(64) != 5
-            a, b = got[sees][:, 2:, others], base[sees][:, 2:, others]
+            others = np.arange(hd) != 5
+            a, b = got[sees][:, nh // 2:, others], base[sees][:, nh // 2:, others]
             assert (np.abs(a - b) <= 2.0 ** -16 + 2 * HALF_STEP[kind] * np.abs(b)).all()   # (added up in another order)
-            assert not np.isfinite(got[sees][:, 2:, 5]).any()
+            assert not np.isfinite(got[sees][:, nh // 2:, 5]).any()
         else:
-            assert np.isnan(got[sees][:, 2:]).all()
+            assert np.isnan(got[sees][:, nh // 2:]).all()
         f.host[name] = clean[name]
     f.rewrite()
 
 
-def test_an_int8_scale_a_row_does_not_see(gv):
+@pytest.mark.parametrize("cache,kind", COMBOS)
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 256), (12, 1, 128), (9, 3, 96), (10, 2, 192), (8, 2, 64), (3, 1, 16)])
+def test_many_columns(gv, cache, kind, nh, nkv, hd):
+    """chains of up to 13 rows: columns that fill one, two and several column tiles, ragged; several chunks"""
+    f = Filled(30, cache, [13, 4, 0, 7, 1], [900, 4, 0, 77, 130], 48, nkv, hd, n_rows=26)
+    _check(gv, f, _queries(31, 26, nh, hd, kind), kind)
+
+
+@pytest.mark.parametrize("n_seqs", [9, 70, 300])
+@pytest.mark.parametrize("cache,kind,rows,nh,nkv,hd", [
+    ("f16", "f32", 1, 8, 4, 64), ("bf16", "bf16", 1, 4, 4, 128), ("i8", "f16", 1, 4, 4, 256), ("f16", "f16", 2, 4, 4, 80),
+    ("bf16", "f32", 1, 4, 4, 192), ("f16", "f32", 6, 16, 4, 64), ("i8", "f32", 6, 16, 4, 16)])
+def test_far_longer_cache_than_sequences(gv, n_seqs, cache, kind, rows, nh, nkv, hd):
+    """a page table for many positions of which most sequences hold few: far more chunks by max_len than there are"""
+    r = np.random.default_rng(32)
+    rows = np.minimum(r.integers(0, rows + 1, n_seqs), rows)
+    lens = np.maximum(rows, r.integers(1, 40, n_seqs))
+    rows[n_seqs // 2], lens[n_seqs // 2] = 1, 700
+    f = Filled(33, cache, rows, lens, 16, nkv, hd)
+    top = 3 * (1 << 20) // n_seqs
+    f.pages = np.concatenate([f.pages, np.full((n_seqs, -(-top // 16) - f.pages.shape[1]), -9, np.int32)], 1)
+    f.batch = gv.PagedBatch(rows, lens, f.pages, max_len=top)
+    q = _queries(34, int(f.start[-1]), nh, hd, kind)
+    _check(gv, f, q, kind)
+    lens = lens.copy()
+    lens[n_seqs - 1] = top + 1
+    f.batch.bufs[1].upload(lens.astype(np.int32))
+    with pytest.raises(gv.GeodeError, match="length"):
+        gv.paged_attention(f.cache, f.batch, q)
+
+
+@pytest.mark.parametrize("nh,hd", [(4, 64), (4, 128), (8, 128), (8, 256)])
+def test_an_int8_scale_a_row_does_not_see(gv, nh, hd):
     """a draft's NaN, infinite or huge scale leaves the rows that do not see it as they were"""
-    f = Filled(14, "i8", [4], [40], 16, 1, 64)
-    q = _queries(15, 4, 4, 64, "f32")
+    f = Filled(14, "i8", [4], [40], 16, 1, hd)
+    q = _queries(15, 4, nh, hd, "f32")
     base, _ = gv.paged_attention(f.cache, f.batch, q)
     sc = f.cache.v_scale.download(np.float32, f.cache.scale_shape)
     p, slot = f.place(0, 38)
