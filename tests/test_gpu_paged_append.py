@@ -123,6 +123,33 @@ def test_prompts(gv, cache, kind, nh, nkv, hd, rope, interleaved):
          interleaved=interleaved)
 
 
+def test_a_pool_past_32_bits(gv):
+    """pages whose elements lie past 2^32 (an 8-bit pool of 5 GB): the same codes and scales as in a small pool"""
+    f = Filled(43, "i8", [3, 1], [70, 9], 64, 2, 128)
+    n_pages = (5 << 30) // (64 * 2 * 128)
+    big = gv.PagedCache(gv.I8, n_pages, 64, 2, 128)
+    moved = np.where(f.pages >= 0, n_pages - 1 - 2 * f.pages, f.pages)
+    r = np.random.default_rng(44)
+    q, k, v = (r.standard_normal((4, h, 128)) for h in (4, 2, 2))
+    cos, sin = _tables(80, 64)
+    a = gv.paged_append(f.cache, f.batch, q, k, v, rope_dim=64, cos=cos, sin=sin)
+    b = gv.paged_append(big, gv.PagedBatch(f.rows, f.lens, moved), q, k, v, rope_dim=64, cos=cos, sin=sin)
+    assert np.array_equal(a, b)
+    size, row = 64 * 2 * 128, gv.DeviceBuffer(64 * 2 * 128)
+    scales = gv.DeviceBuffer(64 * 2 * 4)
+    for i, pos in ((0, 67), (0, 68), (0, 69), (1, 8)):
+        p, s = f.place(i, pos)
+        for small, large, n, buf, t, shape in (
+                (f.cache.k, big.k, size, row, np.int8, (2, 64, 128)), (f.cache.v, big.v, size, row, np.int8, (2, 64, 128)),
+                (f.cache.k_scale, big.k_scale, 512, scales, np.float32, (2, 64)),
+                (f.cache.v_scale, big.v_scale, 512, scales, np.float32, (2, 64))):
+            got = []
+            for src, page in ((small, int(p)), (large, n_pages - 1 - 2 * int(p))):
+                gv.check(gv.lib.gv_memcpy_d2d(buf.ptr, src.ptr + page * n, n), "copy")
+                got.append(buf.download(t, shape)[:, s])
+            assert np.array_equal(*got) and got[0].any()
+
+
 def test_tree_positions_and_far_angles(gv):
     """rotary positions apart from the places in the cache (a draft tree's depths), near the tables' end"""
     pos = np.array([8990, 8991, 8991, 8991, 8992, 8999], np.int32)

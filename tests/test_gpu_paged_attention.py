@@ -199,6 +199,38 @@ def test_equal_calls_give_equal_bits(gv):
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
 
 
+def test_calls_share_a_workspace(gv):
+    """one call after the other in one workspace, nothing waited for in between: what each gives alone; and nothing behind
+    the bytes that were asked for is written"""
+    import ctypes
+
+    nh, hd = 16, 128
+    todo = []
+    for seed, lens, rows in ((40, [3000], [1]), (41, [900, 20, 700], [4, 3, 1]), (42, [5000, 1], [2, 1])):
+        f = Filled(seed, "f16", rows, lens, 32, 2, hd)
+        q = _queries(seed, sum(rows), nh, hd, "f32")
+        todo.append((f, q, gv.paged_attention(f.cache, f.batch, q)))
+    need = [gv.lib.gv_paged_attention_workspace_bytes(ctypes.byref(f.cache.desc), ctypes.byref(f.batch.desc), nh)
+            for f, _, _ in todo]
+    most = max(need)
+    ws = gv.DeviceBuffer(most + 4096)
+    ws.upload(np.full(most + 4096, 0x5A, np.uint8))
+    runs = []
+    for f, q, _ in todo * 2:
+        dq = gv.DeviceBuffer.from_array(q.astype(np.float32))
+        out, lse = gv.DeviceBuffer(q.size * 4), gv.DeviceBuffer(q.shape[0] * nh * 4)
+        runs.append((dq, out, lse))
+        a = gv.GvAttentionRows(type=gv.F32, n_heads=nh, q=dq.ptr, q_row=nh * hd, out=out.ptr, out_row=nh * hd, lse=lse.ptr,
+                               scale=hd ** -0.5)
+        gv.check(gv.lib.gv_paged_attention(ctypes.byref(f.cache.desc), ctypes.byref(f.batch.desc), ctypes.byref(a), ws.ptr,
+                                           most), "gv_paged_attention")
+    gv.check(gv.lib.gv_synchronize(), "gv_synchronize")
+    for (f, q, (want, want_lse)), (_, out, lse) in zip(todo * 2, runs):
+        assert np.array_equal(out.download(np.float32, want.shape), want)
+        assert np.array_equal(lse.download(np.float32, want_lse.shape), want_lse)
+    assert (ws.download(np.uint8, (most + 4096,))[most:] == 0x5A).all()
+
+
 def test_rows_before_and_behind_the_sequences(gv):
     f = Filled(23, "f16", [2, 1], [30, 600], 32, 2, 64, n_rows=9, first_row=2)
     _check(gv, f, _queries(24, 9, 4, 64, "f32"), "f32")
