@@ -93,7 +93,7 @@ __device__ inline void store_logits(float *p, float4 x, int m) {
     }
 }
 
-// Q: quads a thread takes (the slice: Q x 2,048 tokens)
+// Q: quads a thread takes (the slice: Q x 1,024 tokens)
 template <int TYPE, int Q, bool IN_PLACE>
 __global__ __launch_bounds__(kRuleThreads) void logits_rules_kernel(const RuleArgs a) {
     constexpr int S = Q * kRuleQuad;
@@ -267,13 +267,15 @@ extern "C" int gv_process_logits(const gv_logits_rules *rules, const void *logit
                  "logits and out: device memory");
     GV_CHECK_ARG(ld >= V && ldo >= V && ld < int64_t{1} << 36 && ldo < int64_t{1} << 36, "ld and ldo: at least V");
     GV_CHECK_ARG(logits != out || (type == GV_F32 && ld == ldo), "out is logits only with GV_F32 and ldo = ld");
-    GV_CHECK_ARG(!rules->tokens || (rules->begin && rules->end && rules->n_tokens >= 0 && rules->n_tokens <= 1 << 30),
-                 "tokens need begin, end and n_tokens (at most 2^30)");
+    GV_CHECK_ARG(!rules->tokens || (rules->begin && rules->end && rules->n_tokens >= 0 && rules->n_tokens < 1 << 30),
+                 "tokens need begin, end and n_tokens (below 2^30)");
     GV_CHECK_ARG(rules->tokens || !(rules->repetition || rules->frequency || rules->presence), "penalties need tokens");
     GV_CHECK_ARG(!rules->bias_token || (rules->bias_value && rules->bias_begin && rules->bias_end && rules->n_biases >= 0),
                  "biases need bias_value, bias_begin, bias_end and n_biases");
     GV_CHECK_ARG(!rules->masks || (rules->mask_of && rules->n_masks >= 1 && rules->ld_mask >= (V + 31) / 32),
                  "masks need mask_of, n_masks and ld_mask of at least ceil(V / 32)");
+    const int q = rules_quads(rows, V), n_slices = (V + q * kRuleQuad - 1) / (q * kRuleQuad);
+    GV_CHECK_ARG(static_cast<int64_t>(rows) * n_slices < 1 << 24, "too many logits for one call (2^36)");
     if (ensure_init() != 0) return -1;
     OnDevice dev;
     int *faults = queued_faults();
@@ -282,8 +284,7 @@ extern "C" int gv_process_logits(const gv_logits_rules *rules, const void *logit
     a.r = *rules;
     a.logits = static_cast<const char *>(logits), a.out = out;
     a.ld = ld, a.ldo = ldo;
-    const int q = rules_quads(rows, V);
-    a.V = V, a.n_slices = (V + q * kRuleQuad - 1) / (q * kRuleQuad);
+    a.V = V, a.n_slices = n_slices;
     a.faults = faults;
     if (logits == static_cast<const void *>(out)) return launch_rules_q<GV_F32, true>(a, rows, q, stream());
     if (type == GV_F32) return launch_rules_q<GV_F32>(a, rows, q, stream());

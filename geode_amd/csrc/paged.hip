@@ -1,6 +1,7 @@
 // paged.hip - the paged cache of several conversations: new rows' keys and values appended to it (gv_paged_append),
 // and what the paged calls share on the host.
 #include <algorithm>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -23,6 +24,8 @@ int *g_fault_host = nullptr, *g_fault_dev = nullptr;
 }  // namespace
 
 int *queued_faults() {
+    static std::mutex once;   // (calls of several host threads)
+    const std::lock_guard<std::mutex> lock(once);
     if (g_fault_dev) return g_fault_dev;
     void *h = nullptr, *d = nullptr;
     // (portable: any of the process's GPUs may write it; kept until the process ends)
@@ -33,8 +36,8 @@ int *queued_faults() {
         set_error("no pinned memory for the queued calls' faults");
         return nullptr;
     }
+    for (int i = 0; i < kFaultCount; ++i) static_cast<int *>(h)[i] = 0;
     g_fault_host = static_cast<int *>(h);
-    for (int i = 0; i < kFaultCount; ++i) g_fault_host[i] = 0;
     g_fault_dev = static_cast<int *>(d);
     return g_fault_dev;
 }
@@ -87,7 +90,8 @@ int check_kv(const gv_paged_kv *c, const char *call) {
 int check_batch(const gv_paged_batch *b, const gv_paged_kv *c, const char *call) {
     GV_CHECK_ARG(b, "no batch");
     GV_CHECK_ARG(b->n_seqs >= 1 && b->n_seqs <= 1 << 20, "n_seqs: 1 to 2^20");
-    GV_CHECK_ARG(b->n_rows >= 1 && b->n_rows <= 1 << 24, "n_rows: 1 to 2^24");
+    // (a launch's threads along an axis are counted in 32 bits)
+    GV_CHECK_ARG(b->n_rows >= 1 && b->n_rows < 1 << 24, "n_rows: 1 to 2^24 - 1");
     GV_CHECK_ARG(b->max_rows >= 1, "max_rows: at least 1");
     GV_CHECK_ARG(b->row_start && b->lens && b->pages, "row_start, lens and pages are needed");
     GV_CHECK_ARG(b->ld_pages >= 1 && b->ld_pages <= INT32_MAX, "ld_pages: at least 1");
@@ -180,13 +184,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
     Seq s;
     const int i = seq_of_row(a.b, t, s);
     if (i >= a.b.n_seqs) return;   // a row behind the last sequence
-    const int j = t - s.first;
-    if (j < 0 && i == 0) return;   // a row before the first sequence
-    if (!s.fits || j < 0 || j >= s.rows) {
+    if (t < s.first && i == 0) return;   // a row before the first sequence
+    if (!s.fits || t < s.first || t >= s.first + s.rows) {
         if (lane == 0) queue_fault(a.faults, kFaultRows);
         return;
     }
-    const int pos = s.len - s.rows + j;
+    const int pos = s.len - s.rows + t - s.first;
     const int page = a.b.pages[i * a.b.ld_pages + pos / a.kv.page], slot = pos % a.kv.page;
     const int rp = a.positions ? a.positions[t] : pos;
     if (a.half > 0 && (rp < 0 || rp >= a.n_positions)) {

@@ -127,10 +127,20 @@ static size_t attn_ws_bytes(const AttnPlan &p, const gv_paged_kv &kv, const gv_p
            (static_cast<size_t>(kv.head_dim) + 2) * 4;
 }
 
+static int64_t attn_grid(const AttnPlan &p, const gv_paged_kv &kv, const gv_paged_batch &b) {
+    const int64_t units = static_cast<int64_t>(b.n_seqs) * (kv.n_kv_heads / p.inner_heads) * p.n_chunks;
+    return (units + 7) / 8 * 8 * p.col_groups * p.inner_heads;
+}
+
 static int check_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, int n_heads, const char *call) {
     if (check_kv(kv, call) != 0 || check_batch(batch, kv, call) != 0) return -1;
     GV_CHECK_ARG(batch->max_rows <= kAttnMaxRows, "at most 32 rows a sequence");
     GV_CHECK_ARG(n_heads >= 1 && n_heads <= 4096 && n_heads % kv->n_kv_heads == 0, "n_heads: a multiple of n_kv_heads, at most 4096");
+    // (a launch's threads along an axis are counted in 32 bits; the partial results' size in 64, far from their end)
+    const AttnPlan p = attn_plan(*kv, *batch, n_heads);
+    GV_CHECK_ARG(attn_grid(p, *kv, *batch) < 1 << 24 &&
+                     static_cast<int64_t>(p.n_chunks) * batch->n_rows < (int64_t{1} << 46) / (n_heads * int64_t{kv->head_dim + 2} * 4),
+                 "too many sequences, rows, heads and positions for one call");
     return 0;
 }
 
@@ -162,9 +172,6 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
     const size_t need = attn_ws_bytes(p, *kv, *batch, r->n_heads);
     GV_CHECK_ARG(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need),
                  "a 16-byte aligned workspace of gv_paged_attention_workspace_bytes");
-    const int64_t units = static_cast<int64_t>(batch->n_seqs) * (kv->n_kv_heads / p.inner_heads) * p.n_chunks;
-    const int64_t grid = (units + 7) / 8 * 8 * p.col_groups * p.inner_heads;
-    GV_CHECK_ARG(grid < int64_t{1} << 31, "too many sequences, heads and positions for one call");
     if (ensure_init() != 0) return -1;
     OnDevice dev;
     int *faults = queued_faults();
@@ -180,7 +187,7 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
     a.group_inv = 1.0f / static_cast<float>(a.group);
     a.chunk = p.chunk, a.n_chunks = p.n_chunks, a.col_groups = p.col_groups, a.inner_heads = p.inner_heads;
     a.scale = r->scale, a.faults = faults;
-    const unsigned g = static_cast<unsigned>(grid);
+    const unsigned g = static_cast<unsigned>(attn_grid(p, *kv, *batch));
     const int rc = kv->type == GV_F16    ? launch_attn_f16(a, p.ct, g, stream())
                    : kv->type == GV_BF16 ? launch_attn_bf16(a, p.ct, g, stream())
                                          : launch_attn_i8(a, p.ct, g, stream());

@@ -410,7 +410,8 @@ typedef struct gv_paged_kv {
     int32_t n_pages;
     void *k, *v;        /* 16-byte aligned */
     float *k_scale, *v_scale; /* GV_I8: [n_pages][n_kv_heads][page_size], 16-byte aligned; else ignored */
-    int64_t page_stride, head_stride, pos_stride; /* elements, positive multiples of 16; head_stride and pos_stride below 2^24 */
+    int64_t page_stride, head_stride, pos_stride; /* elements, positive multiples of 16; page_stride below 2^40,
+                           head_stride and pos_stride below 2^24, n_kv_heads * head_stride below 2^28 */
 } gv_paged_kv;
 
 /* The rows of one step: sequence i has rows row_start[i] .. row_start[i + 1] - 1 (row_start[0] >= 0, never descending;
@@ -419,7 +420,7 @@ typedef struct gv_paged_kv {
  * pages[i * ld_pages + p / page_size]; entries past the last position are not read. Sequences may share pages that
  * no new row goes to. */
 typedef struct gv_paged_batch {
-    int32_t n_seqs, n_rows;  /* n_rows: the rows the step's arrays hold */
+    int32_t n_seqs, n_rows;  /* n_rows: the rows the step's arrays hold, below 2^24 */
     int32_t max_rows;        /* at least every sequence's rows */
     int32_t max_len;         /* at least every lens[i]; at most ld_pages * page_size */
     const int32_t *row_start;/* [n_seqs + 1] */
@@ -434,18 +435,19 @@ typedef struct gv_paged_batch {
 typedef struct gv_append_rows {
     int32_t type;             /* GV_F32, GV_F16 or GV_BF16: q, k and v */
     int32_t n_heads;          /* query heads, 0: no queries */
-    const void *q, *k, *v;    /* row t's head h at t * q_row + h * q_head (elements, multiples of 4); k, v alike */
+    const void *q, *k, *v;    /* row t's head h at t * q_row + h * q_head (elements, multiples of 4; four elements
+                                 aligned, a row's heads within 2^28 elements); k, v alike */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* (they may be parts of one array, as q | k | v's product) */
-    const float *q_norm, *k_norm; /* [head_dim] or NULL: not normalized */
+    const float *q_norm, *k_norm; /* [head_dim], 16-byte aligned, or NULL: not normalized */
     float eps;
     int32_t rope_dim;         /* a multiple of 8, at most head_dim; 0: no rotation */
     int32_t interleaved;      /* 0: value i turns with value i + rope_dim / 2 (the model's); 1: 2 i with 2 i + 1 */
-    const float *cos, *sin;   /* [n_positions][rope_dim / 2] */
+    const float *cos, *sin;   /* [n_positions][rope_dim / 2], 16-byte aligned */
     int32_t n_positions;
     const int32_t *positions; /* [n_rows] rotary positions (a draft tree's), or NULL: the position in the cache */
     int32_t q_type;           /* GV_F32, GV_F16 or GV_BF16 */
     void *q_out;              /* [n_rows], row t's head h at t * q_out_row + h * head_dim; may be q itself, of the same
-                                 type and layout */
+                                 type and layout; else it overlaps no input */
     int64_t q_out_row;
 } gv_append_rows;
 int gv_paged_append(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv_append_rows *rows);
@@ -453,21 +455,23 @@ int gv_paged_append(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv
 /* Attention of each sequence's rows (at most 32 a sequence) over its cached positions, its own rows' among them:
  * out = sum softmax(scale q . k) v over the positions before the sequence's first new row and, of its new rows, those
  * the row sees: itself and the rows before it, or with `visible` the rows j whose bit j is set. A row that sees
- * nothing gives zeros and lse -inf. What a row does not see does not reach it, NaNs and infinities included. Query head
- * h reads KV head h / (n_heads / n_kv_heads). Scores, softmax and sums in fp32, the weights with at least 16 bits. */
+ * nothing gives zeros and lse -inf. What a row does not see does not reach it, NaNs and infinities included; a NaN key that
+ * it sees makes the head's result NaN, a NaN or infinite value that dim's result not finite, and infinite keys, NaN or
+ * infinite scales of an int8 cache leave the head's result unspecified. Query head h reads KV head h / (n_heads / n_kv_heads). Scores, softmax and sums in fp32, the weights with at
+ * least 16 bits. Equal calls give equal bits. */
 typedef struct gv_attention_rows {
     int32_t type;            /* q and out: the cache's type or GV_F32 (GV_I8: GV_F32, GV_F16 or GV_BF16) */
     int32_t n_heads;         /* a multiple of n_kv_heads */
     const void *q;           /* row t's head h at t * q_row + h * head_dim (elements; 16-byte aligned, q_row a multiple of 8) */
     int64_t q_row;
-    void *out;               /* likewise */
+    void *out;               /* likewise; overlaps no input */
     int64_t out_row;
     float *lse;              /* [n_rows][n_heads] log of the sum of exp(score), or NULL */
     float scale;
     const uint32_t *visible; /* [n_rows] or NULL: a chain */
 } gv_attention_rows;
-/* Scratch of one call (0: none needed, or arguments that the call refuses). Calls may share it: they run one after
- * the other. It holds partial results for max_len positions, whatever the lengths turn out to be. */
+/* Scratch of one call (0: none needed, or arguments that the call refuses). Calls may share it: the library's stream runs
+ * them one after the other. It holds partial results for max_len positions, whatever the lengths turn out to be. */
 size_t gv_paged_attention_workspace_bytes(const gv_paged_kv *kv, const gv_paged_batch *batch, int n_heads);
 int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv_attention_rows *rows, void *ws,
                        size_t ws_bytes);
@@ -483,7 +487,7 @@ int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const
 typedef struct gv_logits_rules {
     const float *repetition, *frequency, *presence; /* [rows] */
     const int32_t *tokens;
-    int64_t n_tokens;                  /* ranges lie within [0, n_tokens); at most 2^30 */
+    int64_t n_tokens;                  /* ranges lie within [0, n_tokens); below 2^30 */
     const int32_t *begin, *generated, *end; /* [rows]; generated NULL: the whole history */
     const int32_t *bias_token;
     const float *bias_value;
@@ -495,7 +499,7 @@ typedef struct gv_logits_rules {
     const int32_t *mask_of;            /* [rows] the row's mask, negative: none */
 } gv_logits_rules;
 /* type: GV_F32, GV_F16 or GV_BF16 of the logits; rows ld (out: ldo) elements apart; out may be logits itself
- * (GV_F32, ldo = ld): what no rule changes is then not written. */
+ * (GV_F32, ldo = ld): what no rule changes is then not written; else the two do not overlap. */
 int gv_process_logits(const gv_logits_rules *rules, const void *logits, int type, int64_t ld, int rows, int V,
                       float *out, int64_t ldo);
 

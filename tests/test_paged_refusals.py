@@ -78,6 +78,22 @@ def test_attention(rows, kv, batch, ws, word):
              "gv_paged_attention", word)
 
 
+def test_more_than_a_launch_can_count():
+    """the threads of a launch's axis past 32 bits, partial results past any memory: refused, not wrapped around"""
+    kv = _kv(n_kv_heads=8, head_dim=256, page_size=64, pos_stride=256, head_stride=16384, page_stride=131072)
+    for b, heads in ((_batch(max_len=1 << 30, ld_pages=1 << 24), 8), (_batch(n_seqs=1 << 20, max_len=1 << 16, ld_pages=1024), 8),
+                     (_batch(n_rows=(1 << 24) - 1, max_len=1 << 29, ld_pages=1 << 23), 4096)):
+        r = _rows(n_heads=heads, q_row=1 << 20, out_row=1 << 20)
+        assert g.lib.gv_paged_attention_workspace_bytes(ctypes.byref(kv), ctypes.byref(b), heads) == 0
+        _refused(g.lib.gv_paged_attention(ctypes.byref(kv), ctypes.byref(b), ctypes.byref(r), MEM, 1 << 62), "too many")
+    b = _batch(n_rows=1 << 24)
+    _refused(g.lib.gv_paged_append(ctypes.byref(_kv()), ctypes.byref(b), ctypes.byref(_append())), "n_rows")
+    rules = g.GvLogitsRules(tokens=MEM, begin=MEM, end=MEM, n_tokens=1 << 30)
+    _refused(g.lib.gv_process_logits(ctypes.byref(rules), 2 * MEM, g.F32, 100, 2, 100, MEM, 100), "n_tokens")
+    _refused(g.lib.gv_process_logits(ctypes.byref(g.GvLogitsRules()), 2 * MEM, g.F32, 1 << 24, 65536, 1 << 24, MEM, 1 << 24),
+             "too many")
+
+
 def test_attention_workspace_too_small():
     b = _batch(max_len=2000, ld_pages=100)
     n = g.lib.gv_paged_attention_workspace_bytes(ctypes.byref(_kv()), ctypes.byref(b), 4)
