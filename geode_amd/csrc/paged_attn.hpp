@@ -150,19 +150,16 @@ __device__ inline uint32_t i8_pair(uint32_t hi, uint32_t lo, uint32_t sel) {
 }
 constexpr float kI8Unit = 512.0f;   // a code's operand x this is the code
 
-// eight consecutive queries' values as floats (TYPE runtime: staging only)
-__device__ inline void load8(const char *p, int type, float (&x)[8]) {
-    if (type == GV_F32) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 16);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const au4 w = *reinterpret_cast<const au4 *>(p);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[2 * k] = type == GV_F16 ? half_lo(w[k]) : bf16_lo(w[k]);
-            x[2 * k + 1] = type == GV_F16 ? half_hi(w[k]) : bf16_hi(w[k]);
-        }
-    }
+// The power of two that a column's int8 weights are divided by, the largest value scale so far below 2 of it: of that scale
+// (at least 2^-113, so that 2^14 over it is a float); 2^14 over it; one over another, the first at most the second.
+constexpr uint32_t kUnitLeast = 14u << 23;
+__device__ inline float unit_of(float scale) {
+    return __uint_as_float(min(max(__float_as_uint(scale) & 0x7F800000u, kUnitLeast), 0x7F000000u));
+}
+__device__ inline float over_unit(float unit) { return __uint_as_float((268u << 23) - __float_as_uint(unit)); }
+__device__ inline float unit_ratio(float a, float b) {
+    const int r = static_cast<int>(0x3F800000u + __float_as_uint(a) - __float_as_uint(b));
+    return r > 0 ? __int_as_float(r) : 0.0f;
 }
 
 // ---------------------------------------------------------------- what both kernels begin with
@@ -290,29 +287,42 @@ struct QueryScale {
 // workgroup; ends with a barrier.
 template <bool BF, bool I8, int QP, int NCH, bool EX, int CT>
 __device__ inline QueryScale stage_queries(const AttnArgs &a, const AttnUnit &u, au4 *lds_q, float *lds_amax) {
-    const int tid = threadIdx.x;
-    const int lane = tid & 63, i16 = lane & 15, g4 = lane >> 4;
-    const QueryScale qs{lds_amax, !BF && a.type != GV_F16};
-    const int qes = a.type == GV_F32 ? 4 : 2;
+    constexpr bool F32 = QP > 1;   // (else one 16-bit type's values: a part)
+    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QueryScale qs{lds_amax, F32 ? !BF : I8 && a.type != GV_F16};
+    constexpr int QU = (CT * NCH + kAttnWaves - 1) / kAttnWaves;
+    au4 raw[QU][F32 ? 2 : 1];
+    uint32_t in = 0;
+#pragma unroll
+    for (int k = 0; k < QU; ++k) {   // (every load on its way before the first is used)
+        const int c = (k * kAttnWaves + wave) % NCH, ct = (k * kAttnWaves + wave) / NCH;
+        const int x = u.q0 + ct * 16 + i16;
+        const int d = I8 ? (c >> 1) * 64 + g4 * 16 + (c & 1) * 8 : c * 32 + g4 * 8;
+        const bool ok = ct < CT && x < u.nq && (EX || d < a.kv.hd);
+        const int xc = ok ? x : 0, r = row_of(a, xc);
+        const au4 *from = reinterpret_cast<const au4 *>(
+            a.q + ((u.s.first + r) * a.q_row + static_cast<int64_t>(u.head * a.group + xc - r * a.group) * a.kv.hd + (ok ? d : 0)) * (F32 ? 4 : 2));
+        raw[k][0] = from[0];
+        if constexpr (F32) raw[k][1] = from[1];
+        if (ok) in |= 1u << k;
+    }
     if (qs.scaled) {
-        for (int i = tid; i < CT * 16; i += kAttnThreads) lds_amax[i] = 0.0f;
+        if (tid < CT * 16) lds_amax[tid] = 0.0f;
         __syncthreads();
     }
-    constexpr int QU = (CT * NCH * 64 + kAttnThreads - 1) / kAttnThreads;
     float qv[QU][8];
 #pragma unroll
     for (int k = 0; k < QU; ++k) {
-        const int w = k * kAttnThreads + tid, c = w / 64 % NCH, ct = w / 64 / NCH;
-        const int x = u.q0 + ct * 16 + i16;
-        const int d = I8 ? (c >> 1) * 64 + g4 * 16 + (c & 1) * 8 : c * 32 + g4 * 8;
-        const bool in = ct < CT && x < u.nq && (EX || d < a.kv.hd);
-        const int xc = in ? x : 0, r = row_of(a, xc);
-        load8(a.q + ((u.s.first + r) * a.q_row + static_cast<int64_t>(u.head * a.group + xc - r * a.group) * a.kv.hd + (in ? d : 0)) * qes,
-              a.type, qv[k]);
+        const bool ok = in >> k & 1;
+        const int ct = (k * kAttnWaves + wave) / NCH;
         float m = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            qv[k][j] = in ? qv[k][j] : 0.0f;
+            const uint32_t w = ok ? raw[k][F32 ? j / 4 : 0][F32 ? j % 4 : j / 2] : 0u;
+            if constexpr (F32) qv[k][j] = __uint_as_float(w);
+            else if (BF || (I8 && a.type == GV_BF16)) qv[k][j] = j & 1 ? bf16_hi(w) : bf16_lo(w);
+            else qv[k][j] = j & 1 ? half_hi(w) : half_lo(w);
             m = fmaxf(m, fabsf(qv[k][j]));
         }
         if (qs.scaled) {   // (positive floats order as their bits)
@@ -323,7 +333,7 @@ __device__ inline QueryScale stage_queries(const AttnArgs &a, const AttnUnit &u,
     if (qs.scaled) __syncthreads();
 #pragma unroll
     for (int k = 0; k < QU; ++k) {
-        const int w = k * kAttnThreads + tid, c = w / 64 % NCH, ct = w / 64 / NCH;
+        const int c = (k * kAttnWaves + wave) % NCH, ct = (k * kAttnWaves + wave) / NCH;
         if (ct >= CT) continue;
         if (qs.scaled) {
             const float f = __uint_as_float(static_cast<uint32_t>(127 + qs.exponent(ct)) << 23);
@@ -443,7 +453,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         sc[ct] = a.scale * qs.undo(ct) * (I8 ? kI8Unit : 1.0f);
-        m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = 0.0f;
+        m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = I8 ? __uint_as_float(kUnitLeast) : 0.0f;
         bits[ct] = seen_rows(a, u, q0 + ct * 16 + i16);
     }
     af4 acc[CT][NT];
@@ -530,24 +540,23 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                     if constexpr (I8) vs[j] = see[ct] >> j & 1 ? vs[j] : 0.0f;
                 }
                 top = fmaxf(top, x[j]);
-                if constexpr (I8) vtop = fmaxf(vtop, vs[j]);
+                if constexpr (I8) vtop = fmaxf(vtop, fabsf(vs[j]));
             }
             top = rows_max(top);
             if constexpr (I8) {   // the weights' power of two: the largest scale so far below 2
-                vtop = rows_max(vtop);
-                vtop = __uint_as_float(min(__float_as_uint(vtop), 0x7F000000u) & 0x7F800000u);
+                vtop = unit_of(rows_max(vtop));
             }
             const float mn = fmaxf(m[ct], top), en = I8 ? fmaxf(ex[ct], vtop) : 0.0f;
             if (__any(mn > m[ct] || en > ex[ct])) {
                 const float gone = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * kLog2e);
                 l[ct] *= gone;
-                const float f = I8 && en > ex[ct] ? gone * (ex[ct] / en) : gone;
+                const float f = I8 && en > ex[ct] ? gone * unit_ratio(ex[ct], en) : gone;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) acc[ct][n] *= f;
                 m[ct] = mn, ex[ct] = en;
             }
             const float base = mn == -INFINITY ? 0.0f : mn;
-            const float up = I8 ? (en > 0.0f ? 16384.0f / en : 0.0f) : 16384.0f;
+            const float up = I8 ? over_unit(en) : 16384.0f;
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -664,7 +673,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
         for (int w = 1; w < kAttnWaves; ++w) mt = fmaxf(mt, lds_m[w][col]), et = fmaxf(et, lds_e[w][col]);
         float f = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mt) * kLog2e);
-        if constexpr (I8) f = et > 0.0f ? f * (ex[ct] / et) : 0.0f;
+        if constexpr (I8) f *= unit_ratio(ex[ct], et);
         float *o = lds_o + (wave * 16 + i16) * OLD;
 #pragma unroll
         for (int r = 0; r < 4; ++r)

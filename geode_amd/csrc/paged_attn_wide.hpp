@@ -129,7 +129,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         sc[ct] = a.scale * qs.undo(ct) * (I8 ? kI8Unit : 1.0f);
-        m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = 0.0f;
+        m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = I8 ? __uint_as_float(kUnitLeast) : 0.0f;
         bits[ct] = seen_rows(a, u, u.q0 + ct * 16 + i16);
     }
     af4 acc[4][CT];
@@ -198,11 +198,11 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
                     seen = use && pos < p1 && (pos < ctx || (bits[ct] >> ((pos - ctx) & 31) & 1));
                     x[r] = seen ? x[r] : -INFINITY;
                 }
-                if constexpr (I8) vtop = fmaxf(vtop, seen ? vsc[r] : 0.0f);
+                if constexpr (I8) vtop = fmaxf(vtop, seen ? fabsf(vsc[r]) : 0.0f);
             }
             sv[ct] = x;
             const float top = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-            if constexpr (I8) vtop = rows_max(vtop);
+            if constexpr (I8) vtop = unit_of(rows_max(vtop));
             if (lane < 16) {
                 lds_max[t & 1][wave][ct * 16 + lane] = top;
                 if constexpr (I8) lds_vmax[t & 1][wave][ct * 16 + lane] = vtop;
@@ -218,21 +218,18 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
             for (int w = 0; w < kAttnWaves; ++w) {
                 mn = fmaxf(mn, lds_max[t & 1][w][ct * 16 + i16]);
-                if constexpr (I8) {   // (a power of two: the largest scale so far below 2 of it)
-                    const uint32_t v = __float_as_uint(lds_vmax[t & 1][w][ct * 16 + i16]);
-                    en = fmaxf(en, __uint_as_float(min(v, 0x7F000000u) & 0x7F800000u));
-                }
+                if constexpr (I8) en = fmaxf(en, lds_vmax[t & 1][w][ct * 16 + i16]);
             }
             if (__any(mn > m[ct] || en > ex[ct])) {
                 const float gone = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * kLog2e);
                 l[ct] *= gone;
-                const float f = I8 && en > ex[ct] ? gone * (ex[ct] / en) : gone;
+                const float f = I8 ? gone * unit_ratio(ex[ct], en) : gone;
 #pragma unroll
                 for (int n = 0; n < 4; ++n) acc[n][ct] *= f;
                 m[ct] = mn, ex[ct] = en;
             }
             const float base = mn == -INFINITY ? 0.0f : mn;
-            const float up = I8 ? (en > 0.0f ? 16384.0f / en : 0.0f) : 16384.0f;
+            const float up = I8 ? over_unit(en) : 16384.0f;
             float x[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -332,20 +329,19 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
         }
     };
 
-    // (each part of a round once in the code: the first time round makes the first scores alone, the last the last product)
+    // (each part of a round once in the code: the first time round makes the first scores alone)
     for (int t = -1;; ++t) {
-        if (t >= 0) __syncthreads();
-        if (t > 0) products(t - 1);
-        if (t == rounds) break;
-        if (t >= 0) {
-            load_v(t);
-            weights(t);
-        }
+        if (t >= 0) weights(t);
         if (t + 1 < rounds) {
             scores(t + 1);
             if (t + 2 < rounds) load_k(t + 2);
         }
+        __syncthreads();
+        if (t >= 0) products(t);
+        if (t + 1 == rounds) break;
+        load_v(t + 1);
     }
+    __syncthreads();   // (the queries' place is used again)
 
     // ---- the sums of weights over the waves; two waves of the same dims added; then out
     float *lds_l = reinterpret_cast<float *>(lds_q);   // [wave][CT * 16] (the queries are done with), then the sums
