@@ -354,6 +354,17 @@ __device__ inline uint32_t seen_rows(const AttnArgs &a, const AttnUnit &u, int x
     return x >= u.nq ? 0u : a.visible ? a.visible[u.s.first + r] : 0xFFFFFFFFu >> (31 - r);
 }
 
+// whether one of 2 N 16-bit values is not finite (their magnitudes' largest, two to a word)
+template <bool BF, int N>
+__device__ inline bool any_not_finite(const uint32_t (&w)[N]) {
+    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+    us2 top = __builtin_bit_cast(us2, w[0] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int k = 1; k < N; ++k) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, w[k] & 0x7FFF7FFFu));
+    const uint32_t t = __builtin_bit_cast(uint32_t, top);
+    return max(t & 0xFFFFu, t >> 16) >= (BF ? 0x7F80u : 0x7C00u);
+}
+
 // ---------------------------------------------------------------- few columns
 // KV: the cache's type. QP, PP: the parts of the queries and of the weights. NT: dim tiles of 16 (head_dim at most
 // 16 NT; EX: exactly). CT: column tiles of 16 queries a workgroup takes.
@@ -607,12 +618,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
-            bool w = false;
-#pragma unroll
-            for (int k = 0; k < VW; ++k) {
-                constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
-                w |= (vr[j][k] & e) == e || (vr[j][k] >> 16 & e) == e;
-            }
+            const bool w = any_not_finite<BF, VW>(vr[j]);
             if (w && pos >= ctx) wild |= 1u << j;
         }
         if (__any(wild != 0))   // wild for every lane if it is for one of the 16 that hold the position's dims

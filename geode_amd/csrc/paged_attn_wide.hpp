@@ -283,11 +283,9 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
                         const int pos = p + 16 * (j / 4) + 4 * g4 + j % 4;
                         const bool hole = pos >= p1 || !(at.usable >> (bit + j / 4) & 1);
 #pragma unroll
-                        for (int i = 0; i < VW; ++i) {
-                            vr[k][j][i] = hole ? 0u : vr[k][j][i];
-                            wild |= pos >= ctx && not_finite<BF>(vr[k][j][i]) != 0;
-                        }
+                        for (int i = 0; i < VW; ++i) vr[k][j][i] = hole ? 0u : vr[k][j][i];
                         if (pos >= ctx) own |= 1u << j;
+                        wild |= pos >= ctx && any_not_finite<BF, VW>(vr[k][j]);
                     }
                     if (__any(wild)) {
                         uint32_t rows[4];
