@@ -283,19 +283,22 @@ struct QueryScale {
     }
     __device__ float undo(int ct) const { return __uint_as_float(static_cast<uint32_t>(127 - exponent(ct)) << 23); }
 };
-// The queries' operands to LDS in the order the products take them, [column tile][part][chunk][lane], by the whole
-// workgroup; ends with a barrier.
-template <bool BF, bool I8, int QP, int NCH, bool EX, int CT>
-__device__ inline QueryScale stage_queries(const AttnArgs &a, const AttnUnit &u, au4 *lds_q, float *lds_amax) {
-    constexpr bool F32 = QP > 1;   // (else one 16-bit type's values: a part)
-    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g4 = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const QueryScale qs{lds_amax, F32 ? !BF : I8 && a.type != GV_F16};
-    constexpr int QU = (CT * NCH + kAttnWaves - 1) / kAttnWaves;
-    au4 raw[QU][F32 ? 2 : 1];
+// The queries as a thread has them on their way: eight values of each of QU columns and 32-dim chunks (QP > 1: fp32, else
+// one 16-bit type's), which of them count. Asked for before the pages are: what is asked for later arrives later.
+template <int QP, int NCH, int CT>
+struct Queries {
+    static constexpr int QU = (CT * NCH + kAttnWaves - 1) / kAttnWaves;
+    au4 raw[QU][QP > 1 ? 2 : 1];
     uint32_t in = 0;
+};
+template <bool I8, int QP, int NCH, bool EX, int CT>
+__device__ inline Queries<QP, NCH, CT> load_queries(const AttnArgs &a, const AttnUnit &u) {
+    constexpr bool F32 = QP > 1;
+    const int lane = threadIdx.x & 63, i16 = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    Queries<QP, NCH, CT> qu;
 #pragma unroll
-    for (int k = 0; k < QU; ++k) {   // (every load on its way before the first is used)
+    for (int k = 0; k < qu.QU; ++k) {
         const int c = (k * kAttnWaves + wave) % NCH, ct = (k * kAttnWaves + wave) / NCH;
         const int x = u.q0 + ct * 16 + i16;
         const int d = I8 ? (c >> 1) * 64 + g4 * 16 + (c & 1) * 8 : c * 32 + g4 * 8;
@@ -303,10 +306,21 @@ __device__ inline QueryScale stage_queries(const AttnArgs &a, const AttnUnit &u,
         const int xc = ok ? x : 0, r = row_of(a, xc);
         const au4 *from = reinterpret_cast<const au4 *>(
             a.q + ((u.s.first + r) * a.q_row + static_cast<int64_t>(u.head * a.group + xc - r * a.group) * a.kv.hd + (ok ? d : 0)) * (F32 ? 4 : 2));
-        raw[k][0] = from[0];
-        if constexpr (F32) raw[k][1] = from[1];
-        if (ok) in |= 1u << k;
+        qu.raw[k][0] = from[0];
+        if constexpr (F32) qu.raw[k][1] = from[1];
+        if (ok) qu.in |= 1u << k;
     }
+    return qu;
+}
+// The queries' operands to LDS in the order the products take them, [column tile][part][chunk][lane], by the whole
+// workgroup; ends with a barrier.
+template <bool BF, bool I8, int QP, int NCH, int CT>
+__device__ inline QueryScale stage_queries(const AttnArgs &a, const Queries<QP, NCH, CT> &qu, au4 *lds_q, float *lds_amax) {
+    constexpr bool F32 = QP > 1;
+    constexpr int QU = Queries<QP, NCH, CT>::QU;
+    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QueryScale qs{lds_amax, F32 ? !BF : I8 && a.type != GV_F16};
     if (qs.scaled) {
         if (tid < CT * 16) lds_amax[tid] = 0.0f;
         __syncthreads();
@@ -314,12 +328,12 @@ __device__ inline QueryScale stage_queries(const AttnArgs &a, const AttnUnit &u,
     float qv[QU][8];
 #pragma unroll
     for (int k = 0; k < QU; ++k) {
-        const bool ok = in >> k & 1;
+        const bool ok = qu.in >> k & 1;
         const int ct = (k * kAttnWaves + wave) / NCH;
         float m = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t w = ok ? raw[k][F32 ? j / 4 : 0][F32 ? j % 4 : j / 2] : 0u;
+            const uint32_t w = ok ? qu.raw[k][F32 ? j / 4 : 0][F32 ? j % 4 : j / 2] : 0u;
             if constexpr (F32) qv[k][j] = __uint_as_float(w);
             else if (BF || (I8 && a.type == GV_BF16)) qv[k][j] = j & 1 ? bf16_hi(w) : bf16_lo(w);
             else qv[k][j] = j & 1 ? half_hi(w) : half_lo(w);
@@ -383,6 +397,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 
     const Seq &s = u.s;
     const int p0 = u.p0, p1 = u.p1, ctx = u.ctx, nq = u.nq, q0 = u.q0, head = u.head;
+    const auto qu = load_queries<I8, QP, NCH, EX, CT>(a, u);
     // the pages of this wave's tiles (lane t: step t / 2, tile t % 2)
     const int tile = p0 + kAttnStep * (wave + kAttnWaves * (lane >> 1)) + 16 * (lane & 1);
     const AttnTiles at = attn_tiles(a, u, tile, (lane >> 1) * kAttnWaves * kAttnStep < a.chunk);
@@ -456,7 +471,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
         load_v(0);
     }
 
-    const QueryScale qs = stage_queries<BF, I8, QP, NCH, EX, CT>(a, u, lds_q, lds_amax);
+    const QueryScale qs = stage_queries<BF, I8, QP, NCH, CT>(a, qu, lds_q, lds_amax);
     const int qes = a.type == GV_F32 ? 4 : 2;
 
     float sc[CT], m[CT], l[CT], ex[CT];   // a column's score factor, maximum, sum; int8: the power of two its weights have

@@ -72,6 +72,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
     const int dq = wave % DW, pg = wave / DW;   // which 64 dims, which of the round's products
     const Seq &s = u.s;
     const int p0 = u.p0, p1 = u.p1, ctx = u.ctx;
+    const auto qu = load_queries<I8, QP, NCH, EX, CT>(a, u);
     // every tile of the chunk a lane (chunks of at most 1,024)
     const AttnTiles at = attn_tiles(a, u, p0 + 16 * lane, 16 * lane < a.chunk);
 
@@ -122,7 +123,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
     };
     const int rounds = (p1 - p0 + kRound - 1) / kRound;
     load_k(0);   // (on its way while the queries are made ready)
-    const QueryScale qs = stage_queries<BF, I8, QP, NCH, EX, CT>(a, u, lds_q, lds_amax);
+    const QueryScale qs = stage_queries<BF, I8, QP, NCH, CT>(a, qu, lds_q, lds_amax);
 
     float sc[CT], m[CT], l[CT], ex[CT];
     uint32_t bits[CT];
