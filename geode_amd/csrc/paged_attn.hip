@@ -102,19 +102,32 @@ static AttnPlan attn_plan(const gv_paged_kv &kv, const gv_paged_batch &b, int n_
     p.col_groups = (cols + 16 * p.ct - 1) / (16 * p.ct);
     const bool wide = p.ct > 1 && kv.head_dim > 64;
     const int64_t items = static_cast<int64_t>(b.n_seqs) * kv.n_kv_heads * p.col_groups;
+    // The chunk whose workgroups end first, by what a workgroup takes: some rounds' time to begin and end, and its chunk's rounds.
+    double best = 0.0;
     if (wide) {
-        // Two workgroups a CU are there at once: the rounds of 64 positions that give each of the 512 the same number, the
-        // lengths of several sequences taken as three fifths of the longest. A workgroup that waits for another's end costs a
-        // whole one's time. Measured, chunks of 256 / 320 / 384 / 512: 32 sequences of up to 4,096 positions and 5 rows (16 heads
-        // of 256, fp16) 43 / 38 / 40 / 48 us; one of 32,001 positions and 17 rows (int8) 60 / 66 / 47 / 58.
-        const int64_t rounds = items * ((b.max_len + 63) / 64) * (b.n_seqs > 1 ? 3 : 5) / 5;
-        const int64_t each = (rounds + 511) / 512;
-        p.chunk = each <= 16 ? static_cast<int>(std::max<int64_t>(2, each)) * 64 : 512;
+        // Rounds of 64 positions, seven to begin and end; the lengths of several sequences taken as three fifths of the longest.
+        // Two workgroups share a CU's units where their LDS and registers leave room (one alone takes 0.82 of the time it takes
+        // beside another). Measured, chunks of 256 / 320 / 384 / 512: 32 sequences of up to 4,096 positions and 5 rows (16 heads
+        // of 256, fp16) 41 / 36 / 38 / 44 us; one of 32,001 positions and 17 rows (int8) 56 / 61 / 45 / 51; chunks of 128 / 256 /
+        // 512: two of 4,406 positions and 22 rows (fp16 queries) 30 / 23 / 27.
+        const bool shared = kv.head_dim == 256 || kv.head_dim <= 128;
+        const int64_t rounds = (static_cast<int64_t>(b.max_len + 63) / 64 * (b.n_seqs > 1 ? 3 : 5) + 4) / 5;
+        for (int r = 2; r <= 8; ++r) {
+            const int64_t a_cu = (items * ((rounds + r - 1) / r) + 255) / 256;
+            const double t = (shared ? a_cu == 1 ? 0.82 : 0.5 * static_cast<double>(a_cu) : static_cast<double>(a_cu)) * (r + 7);
+            if (r == 2 || t < best) best = t, p.chunk = 64 * r;
+        }
     } else {
-        // The longest of 128 .. 512 that still gives every CU two workgroups over max_len: a short cache is cut fine (its time
-        // is latency), and a chunk of 512 writes and reads back a few per cent of the bytes it reads.
-        p.chunk = 512;
-        while (p.chunk > 128 && items * ((b.max_len + p.chunk - 1) / p.chunk) < 512) p.chunk /= 2;
+        // Rounds of 128 positions (32 a wave), four and a half to begin and end; workgroups at once as the kernels' registers
+        // allow. Measured, chunks of 128 / 256 / 512: one sequence of 1,003 positions (16 heads of 256) 10.9 / 12.9 / 16.9 us; 33 of
+        // 2,701 (16 heads of 192, one KV head, fp32 queries) 31 / 27 / 20. A longer chunk leaves a ragged batch's CUs idle.
+        const int hd = kv.head_dim;
+        const int at_once = 256 * (p.ct > 1 ? 2 : hd <= 64 ? 4 : hd <= 128 ? 3 : hd == 256 ? 2 : 1);
+        for (int chunk = 128; chunk <= 512; chunk *= 2) {
+            const int64_t turns = (items * ((b.max_len + chunk - 1) / chunk) + at_once - 1) / at_once;
+            const double t = static_cast<double>(turns) * (chunk / 128 + 4.5);
+            if (chunk == 128 || t < best) best = t, p.chunk = chunk;
+        }
     }
     p.n_chunks = (b.max_len + p.chunk - 1) / p.chunk;
     // (heads inside positions: a head's row of a position shares its cache lines with the next head's)
