@@ -366,6 +366,8 @@ __device__ inline QueryScale stage_queries(const AttnArgs &a, const Queries<QP, 
     __syncthreads();
     return qs;
 }
+// a chunk's maximum for the join, which passes over chunks that have none (a sum that is no number is one to be joined)
+__device__ inline float joined_max(float m, float l) { return l != l && m == -INFINITY ? 0.0f : m; }
 // which of its sequence's rows column x sees
 __device__ inline uint32_t seen_rows(const AttnArgs &a, const AttnUnit &u, int x) {
     const int r = row_of(a, x);
@@ -719,7 +721,8 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
             for (int w = 0; w < kAttnWaves; ++w) {
                 const float mw = lds_m[w][ct * 16 + c];
-                if (mw != -INFINITY) ll += lds_l[w][ct * 16 + c] * __builtin_amdgcn_exp2f((mw - mm) * kLog2e);
+                const float lw = lds_l[w][ct * 16 + c];
+                if (mw != -INFINITY || lw != lw) ll += lw * __builtin_amdgcn_exp2f((mw - mm) * kLog2e);
                 const float4 y = *reinterpret_cast<const float4 *>(lds_o + (w * 16 + c) * OLD + d);
                 v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
             }
@@ -737,7 +740,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
             } else {
                 const int64_t to = (static_cast<int64_t>(u.chunk) * a.b.n_rows + row) * a.nh + hq;
                 store4<GV_F32>(reinterpret_cast<char *>(a.parts + to * a.kv.hd + d), v);
-                if (d == 0) *reinterpret_cast<float2 *>(a.ml + to * 2) = float2{mm, ll};
+                if (d == 0) *reinterpret_cast<float2 *>(a.ml + to * 2) = float2{joined_max(mm, ll), ll};
             }
         }
         __syncthreads();

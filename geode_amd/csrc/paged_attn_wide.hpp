@@ -397,7 +397,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
             else store4<GV_BF16>(dst, v);
         }
         if (dq == 0 && e4 == 0) {
-            if (!whole) *reinterpret_cast<float2 *>(a.ml + to * 2) = float2{m[ct], ll};
+            if (!whole) *reinterpret_cast<float2 *>(a.ml + to * 2) = float2{joined_max(m[ct], ll), ll};
             else if (a.lse) a.lse[static_cast<int64_t>(row) * a.nh + hq] = some ? m[ct] + logf(ll) : -INFINITY;
         }
     }

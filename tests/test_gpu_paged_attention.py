@@ -113,6 +113,25 @@ def test_values_a_row_does_not_see(gv, cache, kind, nh, hd):
     f.rewrite()
 
 
+@pytest.mark.parametrize("cache,kind", [("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("nh,hd", [(4, 64), (16, 64), (4, 128), (16, 128), (4, 256), (16, 256)])
+def test_nan_keys_everywhere_in_a_chunk(gv, cache, kind, nh, hd):
+    """positions whose keys are all NaN, a whole chunk of them or every one a row sees: the rows that see them get NaNs, also
+    where the chunks are joined"""
+    f = Filled(45, cache, [3, 3, 3], [2000, 2000, 300], 16, 2, hd)
+    for i, lo, hi in ((0, 512, 1536), (2, 0, 300)):
+        for pos in range(lo, hi):
+            p, s = f.place(i, pos)
+            f.host["k"][p, 0, s] = np.nan
+    f.rewrite()
+    out, lse = gv.paged_attention(f.cache, f.batch, _queries(46, 9, nh, hd, kind), type_=TYPES[kind])
+    half = nh // 2
+    for rows, finite in ((slice(0, 3), False), (slice(3, 6), True), (slice(6, 9), False)):
+        for x in (out[rows][:, :half], lse[rows][:, :half]):
+            assert np.isfinite(x).all() if finite else np.isnan(x).all()
+        assert np.isfinite(out[rows][:, half:]).all() and np.isfinite(lse[rows][:, half:]).all()
+
+
 @pytest.mark.parametrize("cache,kind", COMBOS)
 @pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 256), (12, 1, 128), (9, 3, 96), (10, 2, 192), (8, 2, 64), (3, 1, 16)])
 def test_many_columns(gv, cache, kind, nh, nkv, hd):
