@@ -469,6 +469,8 @@ class PagedBatch:
     def __init__(self, rows, lens, pages, n_rows=None, max_rows=None, max_len=None, first_row=0):
         rows, lens = np.asarray(rows, np.int32), np.asarray(lens, np.int32)
         pages = np.ascontiguousarray(pages, np.int32)
+        if rows.ndim != 1 or lens.shape != rows.shape or pages.ndim != 2 or len(pages) != len(rows):
+            raise GeodeError("PagedBatch: rows [n], lens [n], pages [n, entries]")
         start = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32) + np.int32(first_row)
         self.bufs = [DeviceBuffer.from_array(a) for a in (start, lens, pages)]
         self.desc = GvPagedBatch(rows.size, int(n_rows if n_rows is not None else start[-1]),
@@ -481,7 +483,15 @@ def paged_append(cache, batch, q, k, v, *, type_=F32, q_type=F32, q_norm=None, k
                  interleaved=False, cos=None, sin=None, positions=None):
     """New rows (float [n_rows, heads, head_dim] each, q None: none) normalized, rotated and appended to a PagedCache;
     the queries as float32 values [n_rows, heads, head_dim]"""
-    T, hd = k.shape[0], cache.desc.head_dim
+    T, hd = batch.desc.n_rows, cache.desc.head_dim
+    for name, x, heads in (("k", k, cache.desc.n_kv_heads), ("v", v, cache.desc.n_kv_heads), ("q", q, None)):
+        if x is not None and np.shape(x) != (T, np.shape(x)[1] if heads is None else heads, hd):
+            raise GeodeError(f"paged_append: {name} is [{T}, heads, {hd}], not {list(np.shape(x))}")
+    for name, x, n in (("q_norm", q_norm, hd), ("k_norm", k_norm, hd), ("positions", positions, T)):
+        if x is not None and np.shape(x) != (n,):
+            raise GeodeError(f"paged_append: {name} is [{n}]")
+    if cos is not None and not np.shape(cos) == np.shape(sin) == (np.shape(cos)[0], rope_dim // 2):
+        raise GeodeError(f"paged_append: cos and sin are [positions, {rope_dim // 2}]")
     dq, dk, dv = (None if x is None else _typed(x, type_) for x in (q, k, v))
     dev = {n: None if a is None else DeviceBuffer.from_array(np.ascontiguousarray(a, t))
            for n, a, t in (("q_norm", q_norm, np.float32), ("k_norm", k_norm, np.float32), ("cos", cos, np.float32),
@@ -503,6 +513,10 @@ def paged_attention(cache, batch, q, *, type_=F32, scale=None, visible=None):
     """Attention of the rows' queries (float [n_rows, heads, head_dim]) over a PagedCache: (out, log-sum-exp) as
     float32; visible: each row's bits of its sequence's rows (None: a chain). Rows of no sequence give zeros."""
     T, nh, hd = q.shape
+    if (T, hd) != (batch.desc.n_rows, cache.desc.head_dim):
+        raise GeodeError(f"paged_attention: q is [{batch.desc.n_rows}, heads, {cache.desc.head_dim}], not {list(q.shape)}")
+    if visible is not None and np.shape(visible) != (T,):
+        raise GeodeError(f"paged_attention: visible is [{T}]")
     dq, out, lse = _typed(q, type_), DeviceBuffer(q.size * np.dtype(_NP_TYPE[type_]).itemsize), DeviceBuffer(T * nh * 4)
     out.zero()
     lse.zero()
@@ -523,12 +537,17 @@ def process_logits(logits, *, type_=F32, tokens=None, begin=None, end=None, gene
     """gv_process_logits of rows of logits (float [rows, V]): the rows after the rules, float32 [rows, V]. The arrays are
     those of gv_logits_rules; masks: uint32 [n_masks, words]."""
     rows, V = logits.shape
-    src = _typed(logits, type_)
-    out = src if in_place else DeviceBuffer(rows * V * 4)
     kinds = dict(repetition=np.float32, frequency=np.float32, presence=np.float32, tokens=np.int32, begin=np.int32,
                  generated=np.int32, end=np.int32, bias_token=np.int32, bias_value=np.float32, bias_begin=np.int32,
                  bias_end=np.int32, masks=np.uint32, mask_of=np.int32)
     given = locals()
+    for n, t in kinds.items():
+        if n not in ("tokens", "bias_token", "bias_value", "masks") and given[n] is not None and np.shape(given[n]) != (rows,):
+            raise GeodeError(f"process_logits: {n} is [{rows}]")
+    if bias_token is not None and np.shape(bias_token) != np.shape(bias_value):
+        raise GeodeError("process_logits: a bias_value for each bias_token")
+    src = _typed(logits, type_)
+    out = src if in_place else DeviceBuffer(rows * V * 4)
     dev = {n: DeviceBuffer.from_array(np.ascontiguousarray(given[n], t)) for n, t in kinds.items() if given[n] is not None}
     r = GvLogitsRules(**{n: b.ptr for n, b in dev.items()}, n_tokens=0 if tokens is None else len(tokens),
                       n_biases=0 if bias_token is None else len(bias_token),

@@ -125,6 +125,30 @@ def test_logits(rules, args, word):
                                      a["V"], a["out"], a["ldo"]), "gv_process_logits", word)
 
 
+def test_the_bindings_arrays():
+    """arrays of other shapes than the batch's and the cache's are refused before anything is uploaded"""
+    from types import SimpleNamespace
+
+    import numpy as np
+
+    cache, batch = SimpleNamespace(desc=_kv()), SimpleNamespace(desc=_batch())
+    z = lambda *s: np.zeros(s, np.float32)   # noqa: E731
+    good = dict(q=z(4, 4, 64), k=z(4, 2, 64), v=z(4, 2, 64))
+    for bad in (dict(k=z(3, 2, 64)), dict(v=z(4, 1, 64)), dict(q=z(4, 4, 32)), dict(q_norm=z(32)), dict(positions=z(3)),
+                dict(rope_dim=32, cos=z(9, 16), sin=z(9, 8)), dict(rope_dim=32, cos=z(9, 8), sin=z(9, 8))):
+        with pytest.raises(g.GeodeError, match="paged_append"):
+            g.paged_append(cache, batch, **{**good, **bad})
+    for q, visible in ((z(3, 4, 64), None), (z(4, 4, 32), None), (z(4, 4, 64), z(3))):
+        with pytest.raises(g.GeodeError, match="paged_attention"):
+            g.paged_attention(cache, batch, q, visible=visible)
+    for bad in (dict(begin=z(3)), dict(mask_of=z(1)), dict(repetition=z(2, 1)), dict(bias_token=z(3), bias_value=z(2))):
+        with pytest.raises(g.GeodeError, match="process_logits"):
+            g.process_logits(z(2, 10), **bad)
+    for rows, lens, pages in (([1, 1], [2], z(2, 1)), ([1, 1], [2, 2], z(1, 2)), ([1], [2], z(1))):
+        with pytest.raises(g.GeodeError, match="PagedBatch"):
+            g.PagedBatch(rows, lens, pages)
+
+
 def test_the_structures_are_the_headers():
     """the ctypes structures' sizes against the C compiler's"""
     import os
