@@ -250,6 +250,20 @@ def test_calls_share_a_workspace(gv):
     assert (ws.download(np.uint8, (most + 4096,))[most:] == 0x5A).all()
 
 
+def test_calls_of_several_threads(gv):
+    """calls of several host threads on data and workspaces of their own"""
+    from concurrent.futures import ThreadPoolExecutor
+
+    todo = []
+    for seed, cache, hd in ((47, "f16", 64), (48, "bf16", 128), (49, "i8", 256), (50, "f16", 80)):
+        f = Filled(seed, cache, [1, 7], [1500, 300], 32, 2, hd)
+        q = _queries(seed, 8, 16, hd, "f32")
+        todo.append((f, q, gv.paged_attention(f.cache, f.batch, q)))
+    with ThreadPoolExecutor(4) as pool:
+        for got, (_, _, want) in zip(pool.map(lambda t: gv.paged_attention(t[0].cache, t[0].batch, t[1]), todo * 6), todo * 6):
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 def test_rows_before_and_behind_the_sequences(gv):
     f = Filled(23, "f16", [2, 1], [30, 600], 32, 2, 64, n_rows=9, first_row=2)
     _check(gv, f, _queries(24, 9, 4, 64, "f32"), "f32")
