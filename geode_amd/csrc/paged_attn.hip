@@ -114,18 +114,20 @@ static AttnPlan attn_plan(const gv_paged_kv &kv, const gv_paged_batch &b, int n_
         const int64_t rounds = (static_cast<int64_t>(b.max_len + 63) / 64 * (b.n_seqs > 1 ? 3 : 5) + 4) / 5;
         for (int r = 2; r <= 8; ++r) {
             const int64_t a_cu = (items * ((rounds + r - 1) / r) + 255) / 256;
-            const double t = (shared ? a_cu == 1 ? 0.82 : 0.5 * static_cast<double>(a_cu) : static_cast<double>(a_cu)) * (r + 7);
+            const double t = (shared ? a_cu == 1 ? 0.82 : 0.5 * static_cast<double>(a_cu) : static_cast<double>(a_cu)) *
+                                 (std::min<int64_t>(r, rounds) + 7) + (b.max_len > 64 * r ? 1.5 : 0.0);
             if (r == 2 || t < best) best = t, p.chunk = 64 * r;
         }
     } else {
-        // Rounds of 128 positions (32 a wave), four and a half to begin and end; workgroups at once as the kernels' registers
-        // allow. Measured, chunks of 128 / 256 / 512: one sequence of 1,003 positions (16 heads of 256) 10.9 / 12.9 / 16.9 us; 33 of
+        // Microseconds: rounds of 128 positions (32 a wave), what it takes to begin and end, and the second launch where chunks
+        // are to be joined; workgroups at once as the kernels' registers allow. Measured, chunks of 128 / 256 / 512: one sequence of 1,003 positions (16 heads of 256) 10.9 / 12.9 / 16.9 us; 33 of
         // 2,701 (16 heads of 192, one KV head, fp32 queries) 31 / 27 / 20. A longer chunk leaves a ragged batch's CUs idle.
         const int hd = kv.head_dim;
         const int at_once = 256 * (p.ct > 1 ? 2 : hd <= 64 ? 4 : hd <= 128 ? 3 : hd == 256 ? 2 : 1);
         for (int chunk = 128; chunk <= 512; chunk *= 2) {
             const int64_t turns = (items * ((b.max_len + chunk - 1) / chunk) + at_once - 1) / at_once;
-            const double t = static_cast<double>(turns) * (chunk / 128 + 4.5);
+            const int rounds = (std::min(chunk, b.max_len) + 127) / 128;
+            const double t = static_cast<double>(turns) * (rounds * (0.4 + 0.0064 * hd) + 4 + 0.019 * hd) + (b.max_len > chunk ? 4.8 : 0.0);
             if (chunk == 128 || t < best) best = t, p.chunk = chunk;
         }
     }

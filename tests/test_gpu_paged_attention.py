@@ -81,6 +81,17 @@ def test_tree_and_rows_that_see_nothing(gv, cache, kind, hd):
     assert not out[7].any() and not out[9].any() and np.isneginf(lse[[7, 9]]).all()
 
 
+@pytest.mark.parametrize("cache,kind", [("f16", "f32"), ("bf16", "bf16"), ("i8", "f32"), ("i8", "bf16")])
+@pytest.mark.parametrize("nh,nkv,hd", [(2, 2, 64), (8, 2, 64), (2, 2, 256), (8, 2, 128), (16, 2, 256), (6, 2, 192)])
+def test_trees_across_chunks(gv, cache, kind, nh, nkv, hd):
+    """a sequence's own rows on both sides of a chunk's end, chunks of which a row sees nothing but single positions"""
+    f = Filled(51, cache, [32, 5, 12, 1], [650, 900, 1029, 641], 48, nkv, hd)
+    r = np.random.default_rng(52)
+    vis = r.integers(0, 2 ** 32, 50, dtype=np.uint64).astype(np.uint32)
+    vis[[3, 33, 40]] = 0
+    _check(gv, f, _queries(53, 50, nh, hd, kind), kind, visible=vis)
+
+
 @pytest.mark.parametrize("cache,kind", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
 @pytest.mark.parametrize("nh,hd", [(4, 64), (16, 64), (4, 128), (16, 128), (16, 96), (4, 256), (16, 256), (16, 192)])
 def test_values_a_row_does_not_see(gv, cache, kind, nh, hd):
