@@ -120,10 +120,11 @@ static AttnPlan attn_plan(const gv_paged_kv &kv, const gv_paged_batch &b, int n_
         }
     } else {
         // Microseconds: rounds of 128 positions (32 a wave), what it takes to begin and end, and the second launch where chunks
-        // are to be joined; workgroups at once as the kernels' registers allow. Measured, chunks of 128 / 256 / 512: one sequence of 1,003 positions (16 heads of 256) 10.9 / 12.9 / 16.9 us; 33 of
-        // 2,701 (16 heads of 192, one KV head, fp32 queries) 31 / 27 / 20. A longer chunk leaves a ragged batch's CUs idle.
+        // are to be joined; workgroups at once as the kernels' registers allow. Measured, chunks of 128 / 256 / 512: one sequence
+        // of 1,003 positions (16 heads of 256) 10.3 / 12.7 / 16.5 us and 4 for the join; 33 of 2,701 (16 heads of 192, one KV head,
+        // fp32 queries) 21 + 6 / 19 + 4 / 17 + 5. A longer chunk leaves a ragged batch's CUs idle.
         const int hd = kv.head_dim;
-        const int at_once = 256 * (p.ct > 1 ? 2 : hd <= 64 ? 4 : hd <= 128 ? 3 : hd == 256 ? 2 : 1);
+        const int at_once = 256 * (p.ct > 1 ? 2 : hd <= 64 ? 4 : hd <= 128 ? 3 : 2);
         for (int chunk = 128; chunk <= 512; chunk *= 2) {
             const int64_t turns = (items * ((b.max_len + chunk - 1) / chunk) + at_once - 1) / at_once;
             const int rounds = (std::min(chunk, b.max_len) + 127) / 128;

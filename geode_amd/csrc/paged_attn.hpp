@@ -71,11 +71,11 @@ constexpr int attn_lds() {
 }
 
 // waves a SIMD a kernel's registers leave room for (asked of the compiler: more, and it spills)
-template <int KV, int NT, bool EX, int CT, bool COUNTED>
+template <int NT, int CT, bool COUNTED>
 constexpr int attn_waves() {
     if (CT > 1) return COUNTED ? 1 : 2;
-    if (COUNTED) return NT == 4 ? 3 : NT == 8 ? 2 : 1;   // (the loop over the units takes a few more)
-    return NT == 4 ? (KV == GV_I8 && !EX ? 3 : 4) : NT == 8 ? 3 : EX ? 2 : 1;
+    if (COUNTED) return NT == 16 ? 1 : 3;   // (the loop over the units takes a few more)
+    return NT == 4 ? 4 : NT == 8 ? 3 : 2;
 }
 
 __device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
@@ -258,6 +258,9 @@ __device__ inline int64_t lane64(int64_t v, int l) {   // lane l's value, unifor
 // Loads from a uniform place plus a lane's 32-bit byte offset and a uniform one: buffer instructions, whose addresses take
 // no vector registers (a 64-bit address a lane and load took up to 40).
 typedef uint32_t au2 __attribute__((ext_vector_type(2)));
+// a lane's offset past the buffer's 2^31 - 1 bytes, for dims past head_dim: the load gives zeros and asks no memory (24 heads of
+// 80: 27.0 -> 25.8 us; 16 heads of 192: 19.2 -> 17.5, with selects in its place before)
+constexpr uint32_t kNowhere = 0x80000000u;
 __device__ inline __amdgpu_buffer_rsrc_t place(const void *p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), static_cast<short>(0), 0x7FFFFFFF, 0x00020000);
 }
@@ -430,8 +433,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                     kf[h][c] = load16(kb, klane + c * per, 0);
                 } else {
                     const int d = I8 ? c * 64 + g4 * 16 : c * 32 + g4 * 8;
-                    const au4 w = load16(kb, d < a.kv.hd ? klane + c * per : 0, 0);
-                    kf[h][c] = d < a.kv.hd ? w : au4{0, 0, 0, 0};
+                    kf[h][c] = load16(kb, d < a.kv.hd ? klane + c * per : kNowhere, 0);
                 }
             }
             if constexpr (I8) {
@@ -444,7 +446,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const auto vb = place(a.kv.v + lane64(toff, 2 * st + h) * ES);
-            const uint32_t lo = EX || i16 * NT < a.kv.hd ? vlane : 0;
+            const uint32_t lo = EX || i16 * NT < a.kv.hd ? vlane : kNowhere;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 uint32_t(&w)[VW] = vr[4 * h + r];
@@ -749,7 +751,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 
 // COUNTED: a workgroup takes one unit after the other of those that the lengths make (attn_unit)
 template <int KV, int QP, int PP, int NT, bool EX, int CT, bool COUNTED>
-__global__ __launch_bounds__(kAttnThreads, (attn_waves<KV, NT, EX, CT, COUNTED>())) void paged_attn_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, (attn_waves<NT, CT, COUNTED>())) void paged_attn_kernel(const AttnArgs a) {
     touch_args(a);
     AttnUnit u;
     if constexpr (!COUNTED) {
@@ -782,14 +784,14 @@ int launch_attn_one(const AttnArgs &a, unsigned grid, hipStream_t st) {
 }
 // The units by max_len, or COUNTED in as many workgroups as are there at once: where there are more than 32 units a CU. An
 // empty workgroup keeps its place for a microsecond, so that a batch with one long sequence spends its time on them: one
-// of 65,537 positions among thirty short ones (24 heads of 80, bf16; 16,000 units, most of them empty) 44 us by max_len,
-// 28 counted; 64 full sequences of 8,192 (8,192 units) 137 and 139. Each unit scans the lengths, so only up to
+// of 65,537 positions among thirty short ones (24 heads of 80, bf16; 16,000 units, most of them empty) 45 us by max_len,
+// 24 counted; 64 full sequences of 8,192 (8,192 units) 137 and 139. Each unit scans the lengths, so only up to
 // kCountSeqs sequences.
 constexpr int kCountUnits = 32 * 256, kCountSeqs = 256;
 template <int KV, int QP, int PP, int NT, bool EX, int CT>
 int launch_attn_few(const AttnArgs &a, unsigned grid, hipStream_t st) {
     if (grid > kCountUnits && a.b.n_seqs <= kCountSeqs)
-        return launch_attn_one<KV, QP, PP, NT, EX, CT, true>(a, 256 * attn_waves<KV, NT, EX, CT, true>(), st);
+        return launch_attn_one<KV, QP, PP, NT, EX, CT, true>(a, 256 * attn_waves<NT, CT, true>(), st);
     return launch_attn_one<KV, QP, PP, NT, EX, CT, false>(a, grid, st);
 }
 }  // namespace gv

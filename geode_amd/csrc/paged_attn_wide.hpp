@@ -94,8 +94,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
                 kf[c] = load16(kb, klane + c * per, 0);
             } else {
                 const int d = I8 ? c * 64 + g4 * 16 : c * 32 + g4 * 8;
-                const au4 w = load16(kb, d < a.kv.hd ? klane + c * per : 0, 0);
-                kf[c] = d < a.kv.hd ? w : au4{0, 0, 0, 0};
+                kf[c] = load16(kb, d < a.kv.hd ? klane + c * per : kNowhere, 0);
             }
         }
         if constexpr (I8) {
@@ -112,7 +111,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const auto vb = place(a.kv.v + lane64(at.off, 4 * t + 2 * (pg * KS + k) + h) * ES);
-                const uint32_t lo = EX || vdim < a.kv.hd ? vlane : 0;
+                const uint32_t lo = EX || vdim < a.kv.hd ? vlane : kNowhere;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     if constexpr (VW == 2) {
@@ -405,7 +404,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
 
 // (two workgroups a CU, where the LDS has room for them and the registers for the compiler)
 template <int KV, int QP, int PP, int NT, bool EX, int CT>
-__global__ __launch_bounds__(kAttnThreads, (NT == 16 && (!EX || QP > 2) ? 1 : 2)) void paged_attn_wide_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, (NT == 16 && (QP > 2 || (!EX && QP > 1)) ? 1 : 2)) void paged_attn_wide_kernel(const AttnArgs a) {
     touch_args(a);
     AttnUnit u;
     if (attn_unit<CT, false>(a, blockIdx.x, u) > 0) attn_many_columns<KV, QP, PP, NT, EX, CT>(a, u);
