@@ -151,17 +151,17 @@ def test_many_columns(gv, cache, kind, nh, nkv, hd):
     _check(gv, f, _queries(31, 26, nh, hd, kind), kind)
 
 
-@pytest.mark.parametrize("n_seqs", [9, 70, 300])
+@pytest.mark.parametrize("n_seqs,by_position", [(9, False), (70, False), (300, False), (9, True), (70, True)])
 @pytest.mark.parametrize("cache,kind,rows,nh,nkv,hd", [
     ("f16", "f32", 1, 8, 4, 64), ("bf16", "bf16", 1, 4, 4, 128), ("i8", "f16", 1, 4, 4, 256), ("f16", "f16", 2, 4, 4, 80),
     ("bf16", "f32", 1, 4, 4, 192), ("f16", "f32", 6, 16, 4, 64), ("i8", "f32", 6, 16, 4, 16)])
-def test_far_longer_cache_than_sequences(gv, n_seqs, cache, kind, rows, nh, nkv, hd):
+def test_far_longer_cache_than_sequences(gv, n_seqs, by_position, cache, kind, rows, nh, nkv, hd):
     """a page table for many positions of which most sequences hold few: far more chunks by max_len than there are"""
     r = np.random.default_rng(32)
     rows = np.minimum(r.integers(0, rows + 1, n_seqs), rows)
     lens = np.maximum(rows, r.integers(1, 40, n_seqs))
     rows[n_seqs // 2], lens[n_seqs // 2] = 1, 700
-    f = Filled(33, cache, rows, lens, 16, nkv, hd)
+    f = Filled(33, cache, rows, lens, 16, nkv, hd, by_position)
     top = 3 * (1 << 20) // n_seqs
     f.pages = np.concatenate([f.pages, np.full((n_seqs, -(-top // 16) - f.pages.shape[1]), -9, np.int32)], 1)
     f.batch = gv.PagedBatch(rows, lens, f.pages, max_len=top)
