@@ -195,8 +195,13 @@ def _tree_bits(case, rows):
 
 
 def prepare(case, seed):
-    if case["op"] == "rules":
-        return _prepare_rules(case, seed)
+    s = _prepare_rules(case, seed) if case["op"] == "rules" else _prepare_paged(case, seed)
+    if own:   # (torch fills the inputs on a stream of its own; the package's waits for no other)
+        torch.cuda.synchronize()
+    return s
+
+
+def _prepare_paged(case, seed):
     t = _tables(case, seed)
     g = _gen(seed, 4)
     T, h, kv, d = t["n_rows"], case["heads"], case["kv_heads"], case["dim"]
@@ -212,6 +217,7 @@ def prepare(case, seed):
             THETA ** (-torch.arange(half, device=DEV, dtype=torch.float64) / max(half, 1))
         s["cos"], s["sin"] = angle.cos().float().contiguous(), angle.sin().float().contiguous()
         s["q_out"] = torch.zeros(T, h * d, dtype=TYPES[case["q_type"]], device=DEV)
+        s["read"] = torch.cuda.Event()
     else:
         s["q"] = (torch.randn(T, h * d, device=DEV, generator=g) * 1.5).to(TYPES[case["q_type"]])
         s["out"] = torch.zeros(T, h * d, dtype=TYPES[case["q_type"]], device=DEV)
@@ -258,6 +264,8 @@ def _prepare_rules(case, seed):
 
 # ------------------------------------------------------------------ one pass
 def run(s):
+    """One pass. With `own` the call is queued on the package's stream, as a program queues the next one behind it: its
+    outputs are whole once that stream has been waited for too (a wait for the whole device)."""
     op = s["case"]["op"]
     if own:
         return {"append": _own_append, "attention": _own_attention, "rules": _own_rules}[op](s)
@@ -432,11 +440,15 @@ def _own_append(s):
                        interleaved=int(case["interleaved"]), cos=s["cos"].data_ptr(), sin=s["sin"].data_ptr(),
                        n_positions=s["t"]["longest"], positions=None, q_type=CODES[case["q_type"]],
                        q_out=s["q_out"].data_ptr(), q_out_row=h * d)
+    if case["type"] == "i8":   # (torch reads the cache on a stream of its own: the pass before has done so)
+        s["read"].synchronize()
     g.check(g.lib.gv_paged_append(ctypes.byref(s["kv"]), ctypes.byref(s["batch"]), ctypes.byref(a)), "gv_paged_append")
     if case["type"] == "i8":
-        g.check(g.lib.gv_synchronize(), "gv_synchronize")   # (torch reads the cache on a stream of its own)
+        g.check(g.lib.gv_synchronize(), "gv_synchronize")
         _, _, page, slot = _places(s)
-        return (s["q_out"],) + _int8_values(s, page, slot)
+        values = _int8_values(s, page, slot)
+        s["read"].record()
+        return (s["q_out"],) + values
     return s["q_out"], s["cache"]["k"], s["cache"]["v"]
 
 
