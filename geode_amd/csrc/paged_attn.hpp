@@ -19,7 +19,8 @@
 // values exactly (int8: as fp16 (code) / 512); products are summed in fp32. A query exact in the cache's type is one
 // part; the weights are two parts for 16-bit results (an error of 2^-16 at most, far below the result's own rounding)
 // and 22 or 24 bits for fp32 ones. fp16 parts are taken of values scaled by powers of two (queries by their row's
-// largest value, weights by 2^14), so that neither overflows nor falls below fp16's range.
+// largest value, weights by 2^14, an int8 cache's weights x value scales by their largest's: weight_factor), so that neither
+// overflows nor, where it counts, falls below fp16's range.
 // The weights' exponential takes the difference to the maximum: exp2((s - m) log2 e), accurate whatever the scores' size.
 //
 // Bound by the bytes of keys and values where there are many (131,073 positions, 2 KV heads of 256, fp16, 268 MB: 51 us; 64
@@ -58,7 +59,6 @@ struct AttnArgs {
     int *faults;
 };
 
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kAttnThreads = 256, kAttnWaves = 4, kAttnStep = 32;
 constexpr int kAttnMaxRows = 32;
 
@@ -154,16 +154,20 @@ __device__ inline uint32_t i8_pair(uint32_t hi, uint32_t lo, uint32_t sel) {
 }
 constexpr float kI8Unit = 512.0f;   // a code's operand x this is the code
 
-// The power of two that a column's int8 weights are divided by, the largest value scale so far below 2 of it: of that scale
-// (at least 2^-113, so that 2^14 over it is a float); 2^14 over it; one over another, the first at most the second.
-constexpr uint32_t kUnitLeast = 14u << 23;
-__device__ inline float unit_of(float scale) {
-    return __uint_as_float(min(max(__float_as_uint(scale) & 0x7F800000u, kUnitLeast), 0x7F000000u));
+// An int8 cache's weights take the value scales with them, times a power of two that brings a column's largest weight x scale
+// to 2^13 .. 2^14 (of all scales, whatever their weight, it would push the weights that count below fp16's range). top: log2 of
+// the largest weight x scale before the weights' division by e^m, m the largest score; the factor is held between 2^-114 and
+// 2^126 (weights x scales below 2^-113 lose bits). Nothing seen yet: top and m are -inf, their difference no number, the
+// factor the largest.
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMostFactor = 126;
+__device__ inline float weight_factor(float top, float m) {
+    const float e = fminf(fmaxf(floorf(__builtin_fmaf(-m, kLog2e, top)), 13.0f - kMostFactor), 127.0f);
+    return __builtin_amdgcn_ldexpf(1.0f, 13 - static_cast<int>(e));
 }
-__device__ inline float over_unit(float unit) { return __uint_as_float((268u << 23) - __float_as_uint(unit)); }
-__device__ inline float unit_ratio(float a, float b) {
-    const int r = static_cast<int>(0x3F800000u + __float_as_uint(a) - __float_as_uint(b));
-    return r > 0 ? __int_as_float(r) : 0.0f;
+// log2 of one power of two over another
+__device__ inline float log2_ratio(float a, float b) {
+    return static_cast<float>((__float_as_int(a) - __float_as_int(b)) >> 23);
 }
 
 // ---------------------------------------------------------------- what both kernels begin with
@@ -400,7 +404,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
     constexpr int VW = NT * ES / 4;        // words a lane a V row
     extern __shared__ au4 lds_q[];         // [CT][QP][NCH][64]
     __shared__ float lds_amax[CT * 16];
-    __shared__ float lds_m[kAttnWaves][CT * 16], lds_l[kAttnWaves][CT * 16], lds_e[kAttnWaves][CT * 16];
+    __shared__ float lds_m[kAttnWaves][CT * 16], lds_l[kAttnWaves][CT * 16];
     const int lane = threadIdx.x & 63, i16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));   // (uniform: its branches are)
 
@@ -482,12 +486,13 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
     const QueryScale qs = stage_queries<BF, I8, QP, NCH, CT>(a, qu, lds_q, lds_amax);
     const int qes = a.type == GV_F32 ? 4 : 2;
 
-    float sc[CT], m[CT], l[CT], ex[CT];   // a column's score factor, maximum, sum; int8: the power of two its weights have
+    float sc[CT], m[CT], l[CT];           // a column's score factor, maximum, sum
+    float most[CT], up[CT];               // its weights' factor for the products; int8: log2 of the largest weight x scale e^m
     uint32_t bits[CT];                    // which of the sequence's rows it sees
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         sc[ct] = a.scale * qs.undo(ct) * (I8 ? kI8Unit : 1.0f);
-        m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = I8 ? __uint_as_float(kUnitLeast) : 0.0f;
+        m[ct] = most[ct] = -INFINITY, l[ct] = 0.0f, up[ct] = I8 ? weight_factor(-INFINITY, -INFINITY) : 16384.0f;
         bits[ct] = seen_rows(a, u, q0 + ct * 16 + i16);
     }
     af4 acc[CT][NT];
@@ -550,6 +555,10 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
         }
         uint32_t see[CT];   // (bit j: the lane's column sees its position j)
         au4 pb[CT][PP];
+        float vlog[8];
+        if constexpr (I8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vlog[j] = __builtin_amdgcn_logf(fabsf(vsc[j / 4][j % 4]));
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             float x[8], vs[8];
@@ -563,7 +572,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                     if (seen && !(hole >> j & 1)) see[ct] |= 1u << j;
                 }
             }
-            float top = -INFINITY, vtop = 0.0f;
+            float top = -INFINITY, wtop = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float f = sc[ct];
@@ -574,33 +583,35 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                     if constexpr (I8) vs[j] = see[ct] >> j & 1 ? vs[j] : 0.0f;
                 }
                 top = fmaxf(top, x[j]);
-                if constexpr (I8) vtop = fmaxf(vtop, fabsf(vs[j]));
+                if constexpr (I8) wtop = fmaxf(wtop, __builtin_fmaf(x[j], kLog2e, vlog[j]));
             }
             top = rows_max(top);
-            if constexpr (I8) {   // the weights' power of two: the largest scale so far below 2
-                vtop = unit_of(rows_max(vtop));
-            }
-            const float mn = fmaxf(m[ct], top), en = I8 ? fmaxf(ex[ct], vtop) : 0.0f;
-            if (__any(mn > m[ct] || en > ex[ct])) {
-                const float gone = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * kLog2e);
-                l[ct] *= gone;
-                const float f = I8 && en > ex[ct] ? gone * unit_ratio(ex[ct], en) : gone;
+            if constexpr (I8) wtop = rows_max(wtop);
+            const float mn = fmaxf(m[ct], top), wn = I8 ? fmaxf(most[ct], wtop) : -INFINITY;
+            if (__any(mn > m[ct] || wn > most[ct])) {
+                const float down = mn == -INFINITY ? 0.0f : (m[ct] - mn) * kLog2e;
+                float f = __builtin_amdgcn_exp2f(down);
+                l[ct] *= f;
+                if constexpr (I8) {   // (at most about 2, whatever its two parts are)
+                    const float now = weight_factor(wn, mn);
+                    f = __builtin_amdgcn_exp2f(down + log2_ratio(now, up[ct]));
+                    most[ct] = wn, up[ct] = now;
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) acc[ct][n] *= f;
-                m[ct] = mn, ex[ct] = en;
+                m[ct] = mn;
             }
             const float base = mn == -INFINITY ? 0.0f : mn;
-            const float up = I8 ? over_unit(en) : 16384.0f;
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 x[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
                 sum += x[j];
-                if constexpr (I8) {
-                    x[j] *= vs[j] * up;
+                if constexpr (I8) {   // (weight x scale first: the scale alone may be far above the largest of them)
+                    x[j] = x[j] * vs[j] * up[ct];
                     if constexpr (tail) x[j] = see[ct] >> j & 1 ? x[j] : 0.0f;
                 } else if constexpr (!BF) {
-                    x[j] *= up;
+                    x[j] *= up[ct];
                 }
             }
             l[ct] += sum;
@@ -690,7 +701,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         l[ct] = rows_sum(l[ct]);
-        if (lane < 16) lds_m[wave][ct * 16 + lane] = m[ct], lds_l[wave][ct * 16 + lane] = l[ct], lds_e[wave][ct * 16 + lane] = ex[ct];
+        if (lane < 16) lds_m[wave][ct * 16 + lane] = m[ct], lds_l[wave][ct * 16 + lane] = l[ct];
     }
     __syncthreads();
     const bool whole = s.len <= a.chunk;
@@ -698,11 +709,12 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
     for (int ct = 0; ct < CT; ++ct) {
         if (q0 + ct * 16 >= nq) break;
         const int col = ct * 16 + i16;
-        float mt = lds_m[0][col], et = lds_e[0][col];
+        float mt = lds_m[0][col];
 #pragma unroll
-        for (int w = 1; w < kAttnWaves; ++w) mt = fmaxf(mt, lds_m[w][col]), et = fmaxf(et, lds_e[w][col]);
-        float f = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mt) * kLog2e);
-        if constexpr (I8) f *= unit_ratio(ex[ct], et);
+        for (int w = 1; w < kAttnWaves; ++w) mt = fmaxf(mt, lds_m[w][col]);
+        // (int8: each wave's own factor taken out, so that the sums are the values')
+        const float out_log = I8 ? log2_ratio(kI8Unit, up[ct]) : 0.0f;
+        const float f = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mt) * kLog2e + out_log);
         float *o = lds_o + (wave * 16 + i16) * OLD;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -715,9 +727,9 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
             const int c = e / (NT * 4), d = e % (NT * 4) * 4;
             const int x = q0 + ct * 16 + c;
             if (x >= nq || (!EX && d >= a.kv.hd)) continue;
-            float mm = lds_m[0][ct * 16 + c], ee = lds_e[0][ct * 16 + c];
+            float mm = lds_m[0][ct * 16 + c];
 #pragma unroll
-            for (int w = 1; w < kAttnWaves; ++w) mm = fmaxf(mm, lds_m[w][ct * 16 + c]), ee = fmaxf(ee, lds_e[w][ct * 16 + c]);
+            for (int w = 1; w < kAttnWaves; ++w) mm = fmaxf(mm, lds_m[w][ct * 16 + c]);
             float ll = 0.0f;
             float4 v = float4{0, 0, 0, 0};
 #pragma unroll
@@ -729,7 +741,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                 v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
             }
             const int r = row_of(a, x), row = s.first + r, hq = head * a.group + x - r * a.group;
-            const float unit_v = BF ? 1.0f : I8 ? ee * (kI8Unit / 16384.0f) : 1.0f / 16384.0f;
+            const float unit_v = BF || I8 ? 1.0f : 1.0f / 16384.0f;
             v.x *= unit_v, v.y *= unit_v, v.z *= unit_v, v.w *= unit_v;
             if (whole) {
                 if (ll > 0.0f || ll != ll) v = float4{v.x / ll, v.y / ll, v.z / ll, v.w / ll};

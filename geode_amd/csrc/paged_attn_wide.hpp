@@ -69,7 +69,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
     constexpr int kRound = 64;
     extern __shared__ au4 lds_q[];         // [CT][QP][NCH][64], then the weights [2][2][CT][PP][64]
     au4 *lds_p = lds_q + CT * QP * NCH * 64;
-    __shared__ float lds_amax[CT * 16], lds_max[2][kAttnWaves][CT * 16], lds_vmax[I8 ? 2 : 1][kAttnWaves][CT * 16];
+    __shared__ float lds_amax[CT * 16], lds_max[2][kAttnWaves][CT * 16], lds_wmax[I8 ? 2 : 1][kAttnWaves][CT * 16];
     const int lane = threadIdx.x & 63, i16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int dq = wave % DW, pg = wave / DW;   // which 64 dims, which of the round's products
@@ -127,12 +127,12 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
     load_k(0);   // (on its way while the queries are made ready)
     const QueryScale qs = stage_queries<BF, I8, QP, NCH, CT>(a, qu, lds_q, lds_amax);
 
-    float sc[CT], m[CT], l[CT], ex[CT];
+    float sc[CT], m[CT], l[CT], most[CT], up[CT];   // (as there)
     uint32_t bits[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         sc[ct] = a.scale * qs.undo(ct) * (I8 ? kI8Unit : 1.0f);
-        m[ct] = -INFINITY, l[ct] = 0.0f, ex[ct] = I8 ? __uint_as_float(kUnitLeast) : 0.0f;
+        m[ct] = most[ct] = -INFINITY, l[ct] = 0.0f, up[ct] = I8 ? weight_factor(-INFINITY, -INFINITY) : 16384.0f;
         bits[ct] = seen_rows(a, u, u.q0 + ct * 16 + i16);
     }
     af4 acc[4][CT];
@@ -180,35 +180,34 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
         }
         const int p = p0 + kRound * t + 16 * wave;
         const bool use = at.usable >> (4 * t + wave) & 1, tail = p + 16 > ctx || !use;   // (uniform)
-        float f[4];
+        float f[4], vlog[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             f[r] = I8 ? ksc[r] : 1.0f;
-            if constexpr (I8) vsc[r] = vsc_next[r];
+            if constexpr (I8) vsc[r] = vsc_next[r], vlog[r] = __builtin_amdgcn_logf(fabsf(vsc[r]));
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             af4 x = part[ct][0];
 #pragma unroll
             for (int q = 1; q < QP; ++q) x += part[ct][q];
-            float vtop = 0.0f;
+            float wtop = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 x[r] *= I8 ? sc[ct] * f[r] : sc[ct];
-                bool seen = true;
                 if (tail) {
                     const int pos = p + 4 * g4 + r;
-                    seen = use && pos < p1 && (pos < ctx || (bits[ct] >> ((pos - ctx) & 31) & 1));
+                    const bool seen = use && pos < p1 && (pos < ctx || (bits[ct] >> ((pos - ctx) & 31) & 1));
                     x[r] = seen ? x[r] : -INFINITY;
                 }
-                if constexpr (I8) vtop = fmaxf(vtop, seen ? fabsf(vsc[r]) : 0.0f);
+                if constexpr (I8) wtop = fmaxf(wtop, __builtin_fmaf(x[r], kLog2e, vlog[r]));
             }
             sv[ct] = x;
             const float top = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-            if constexpr (I8) vtop = unit_of(rows_max(vtop));
+            if constexpr (I8) wtop = rows_max(wtop);
             if (lane < 16) {
                 lds_max[t & 1][wave][ct * 16 + lane] = top;
-                if constexpr (I8) lds_vmax[t & 1][wave][ct * 16 + lane] = vtop;
+                if constexpr (I8) lds_wmax[t & 1][wave][ct * 16 + lane] = wtop;
             }
         }
     };
@@ -217,32 +216,36 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
         const bool tail = p0 + kRound * t + 16 * wave + 16 > ctx || !(at.usable >> (4 * t + wave) & 1);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            float mn = m[ct], en = ex[ct];
+            float mn = m[ct], wn = most[ct];
 #pragma unroll
             for (int w = 0; w < kAttnWaves; ++w) {
                 mn = fmaxf(mn, lds_max[t & 1][w][ct * 16 + i16]);
-                if constexpr (I8) en = fmaxf(en, lds_vmax[t & 1][w][ct * 16 + i16]);
+                if constexpr (I8) wn = fmaxf(wn, lds_wmax[t & 1][w][ct * 16 + i16]);
             }
-            if (__any(mn > m[ct] || en > ex[ct])) {
-                const float gone = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * kLog2e);
-                l[ct] *= gone;
-                const float f = I8 ? gone * unit_ratio(ex[ct], en) : gone;
+            if (__any(mn > m[ct] || wn > most[ct])) {
+                const float down = mn == -INFINITY ? 0.0f : (m[ct] - mn) * kLog2e;
+                float f = __builtin_amdgcn_exp2f(down);
+                l[ct] *= f;
+                if constexpr (I8) {
+                    const float now = weight_factor(wn, mn);
+                    f = __builtin_amdgcn_exp2f(down + log2_ratio(now, up[ct]));
+                    most[ct] = wn, up[ct] = now;
+                }
 #pragma unroll
                 for (int n = 0; n < 4; ++n) acc[n][ct] *= f;
-                m[ct] = mn, ex[ct] = en;
+                m[ct] = mn;
             }
             const float base = mn == -INFINITY ? 0.0f : mn;
-            const float up = I8 ? over_unit(en) : 16384.0f;
             float x[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 x[r] = __builtin_amdgcn_exp2f((sv[ct][r] - base) * kLog2e);
                 l[ct] += x[r];
                 if constexpr (I8) {
-                    const float w = x[r] * (vsc[r] * up);
+                    const float w = x[r] * vsc[r] * up[ct];
                     x[r] = tail && sv[ct][r] == -INFINITY ? 0.0f : w;   // (a scale that is not seen may be anything)
                 } else if constexpr (!BF) {
-                    x[r] *= up;
+                    x[r] *= up[ct];
                 }
             }
             uint2 part[PP];
@@ -377,7 +380,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
         for (int w = 0; w < kAttnWaves; ++w) ll += lds_l[w * CT * 16 + ct * 16 + c16];
         const int xr = row_of(a, x), row = s.first + xr, hq = u.head * a.group + x - xr * a.group;
-        const float unit_v = BF ? 1.0f : I8 ? ex[ct] * (kI8Unit / 16384.0f) : 1.0f / 16384.0f;
+        const float unit_v = BF ? 1.0f : I8 ? kI8Unit / up[ct] : 1.0f / 16384.0f;
         const bool some = ll > 0.0f || ll != ll;
         const int64_t to = (static_cast<int64_t>(u.chunk) * a.b.n_rows + row) * a.nh + hq;
 #pragma unroll
