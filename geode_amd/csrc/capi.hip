@@ -163,7 +163,7 @@ int gv_memcpy_d2h(void *dst, const void *src, size_t bytes) {
     if (ensure_init() != 0) return -1;
     GV_CHECK_HIP(hipMemcpyAsync(dst, src, bytes, hipMemcpyDeviceToHost, stream()));
     GV_CHECK_HIP(hipStreamSynchronize(stream()));
-    return 0;
+    return take_queued_faults();
 }
 
 int gv_memcpy_d2d(void *dst, const void *src, size_t bytes) {

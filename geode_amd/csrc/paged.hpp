@@ -14,11 +14,12 @@
 namespace gv {
 
 // ---------------------------------------------------------------- faults met in device memory
-// A kernel that meets one sets its word in pinned host memory (a plain store: every writer writes 1); gv_synchronize
-// reads the words once the stream is idle, clears them and fails.
+// A kernel that meets one sets its word in pinned host memory (every writer writes 1, past the caches: a volatile store); the
+// calls that wait and hand out results (gv_synchronize, gv_memcpy_d2h, the sampling and acceptance calls) read the words
+// behind their wait, clear them and fail.
 enum QueuedFault { kFaultRows = 0, kFaultPage = 1, kFaultPosition = 2, kFaultRange = 3, kFaultCount = 4 };
 int *queued_faults();        // the words as the device addresses them (null: no memory, the error set)
-int take_queued_faults();    // 0, or -1 and a message, the words cleared (the stream idle)
+int take_queued_faults();    // 0, or -1 and a message, the words cleared (behind a wait for the stream)
 __device__ inline void queue_fault(int *words, int kind) {
     *reinterpret_cast<volatile int *>(words + kind) = 1;
 }

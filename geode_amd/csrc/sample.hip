@@ -42,6 +42,7 @@
 #include "../../include/geode_verify.h"
 #include "common.hpp"
 #include "kernels.hpp"
+#include "paged.hpp"
 
 namespace gv {
 namespace {
@@ -1971,6 +1972,7 @@ int gv_sample_rows(const float *logits, int64_t ld, int rows, int V, float tempe
     if (nuclei(rs, rows, temperature, top_p, top_k, cap, c.ws, st) != 0) return -1;
     GV_CHECK_HIP(hipMemcpyAsync(pin, c.ws.picks, 4 * static_cast<size_t>(rows), hipMemcpyDeviceToHost, st));
     GV_CHECK_HIP(hipStreamSynchronize(st));
+    if (take_queued_faults() != 0) return -1;
     std::copy(reinterpret_cast<int32_t *>(pin), reinterpret_cast<int32_t *>(pin) + rows, out);
     return 0;
 }
@@ -2057,7 +2059,7 @@ int gv_accept_match_ex(float *logits, int64_t ld, int V, const int32_t *batch, i
                                done, seq);
         }
         GV_CHECK_HIP(hipGetLastError());
-        if (wait_posted(done, seq, st) != 0) return -1;
+        if (wait_posted(done, seq, st) != 0 || take_queued_faults() != 0) return -1;
         const int emitted = hint[32];
         if (emitted > 0) {
             for (int i = 0; i < emitted; ++i) out[i] = hint[i];
@@ -2085,6 +2087,7 @@ int gv_accept_match_ex(float *logits, int64_t ld, int V, const int32_t *batch, i
         GV_CHECK_HIP(hipGetLastError());
         GV_CHECK_HIP(hipMemcpyAsync(hint, dout, 36 * 4, hipMemcpyDeviceToHost, st));
         GV_CHECK_HIP(hipStreamSynchronize(st));
+        if (take_queued_faults() != 0) return -1;
         const int emitted = hint[32];
         if (emitted > 0) {
             for (int i = 0; i < emitted; ++i) out[i] = hint[i];
@@ -2100,6 +2103,7 @@ int gv_accept_match_ex(float *logits, int64_t ld, int V, const int32_t *batch, i
     GV_CHECK_HIP(hipGetLastError());
     GV_CHECK_HIP(hipMemcpyAsync(hint, dout, 36 * 4, hipMemcpyDeviceToHost, st));
     GV_CHECK_HIP(hipStreamSynchronize(st));
+    if (take_queued_faults() != 0) return -1;
     const int emitted = hint[32];
     for (int i = 0; i < emitted; ++i) out[i] = hint[i];
     if (kept) *kept = hint[33];
@@ -2144,7 +2148,7 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
         hipLaunchKernelGGL(greedy_finish, dim3(1), dim3(kSortThreads), 0, st, c.ws, rs.S, k, hout, hout + 32, done,
                            seq);
         GV_CHECK_HIP(hipGetLastError());
-        if (wait_posted(done, seq, st) != 0) return -1;
+        if (wait_posted(done, seq, st) != 0 || take_queued_faults() != 0) return -1;
         const int emitted = hout[32];
         for (int i = 0; i < emitted; ++i) out[i] = hout[i];
         return emitted;
@@ -2170,7 +2174,7 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
         hipLaunchKernelGGL(fast_textbook, dim3(1), dim3(kSortThreads), lds_t, st, rs, c.ws, k, temperature, fu, hout,
                            hout + 32, done, seq);
         GV_CHECK_HIP(hipGetLastError());
-        if (wait_posted(done, seq, st) != 0) return -1;
+        if (wait_posted(done, seq, st) != 0 || take_queued_faults() != 0) return -1;
         const int emitted = hout[32];
         if (emitted > 0) {
             for (int i = 0; i < emitted; ++i) out[i] = hout[i];
@@ -2187,6 +2191,7 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
     GV_CHECK_HIP(hipGetLastError());
     GV_CHECK_HIP(hipMemcpyAsync(hout, dout, 33 * 4, hipMemcpyDeviceToHost, st));
     GV_CHECK_HIP(hipStreamSynchronize(st));
+    if (take_queued_faults() != 0) return -1;
     const int emitted = hout[32];
     for (int i = 0; i < emitted; ++i) out[i] = hout[i];
     return emitted;

@@ -33,11 +33,12 @@ int gv_device_count(void);
 void *gv_malloc(size_t bytes); /* device memory, NULL on failure */
 int gv_free(void *p);
 int gv_memcpy_h2d(void *dst, const void *src, size_t bytes);
-int gv_memcpy_d2h(void *dst, const void *src, size_t bytes);
+int gv_memcpy_d2h(void *dst, const void *src, size_t bytes); /* waits; fails as gv_synchronize does */
 int gv_memcpy_d2d(void *dst, const void *src, size_t bytes);
 int gv_memset(void *dst, int value, size_t bytes);
-/* Waits for the library's stream. Fails when a call queued since the last one met a fault in device memory (the paged
- * calls and gv_process_logits below). */
+/* Waits for the library's stream. Fails when a queued call met a fault in device memory (the paged calls and
+ * gv_process_logits below) that no call has told yet: the first that waits and hands out results does, once - this one,
+ * gv_memcpy_d2h, gv_sample_rows or a gv_accept call. */
 int gv_synchronize(void);
 /* milliseconds between two points of the library's stream: gv_event_record returns an id */
 int gv_event_record(void);
@@ -395,7 +396,8 @@ int gv_sampler_paths(int64_t *candidate, int64_t *walks);
  * What the host passes is checked by the call (nonzero, gv_last_error). What lies in device memory is checked on the
  * device: a sequence whose row starts or length do not fit, a page outside the pool, a rotary position outside the
  * tables, a token range or mask outside its array. Nothing outside the arrays is read or written for it, what it
- * gives is unspecified, the other sequences and rows are unaffected, and the next gv_synchronize fails with a message. */
+ * gives is unspecified, the other sequences and rows are unaffected, and the next call that waits and hands out results
+ * (gv_synchronize, gv_memcpy_d2h, gv_sample_rows, the gv_accept calls, which then give nothing) fails with a message. */
 enum { GV_F32 = 0, GV_F16 = 1, GV_BF16 = 2, GV_I8 = 3 }; /* element types */
 
 /* One layer's paged cache: n_pages pages of page_size positions, keys and values apart. The element (page, head,

@@ -1,0 +1,85 @@
+"""What a fault met in device memory reaches: every call that waits and hands out results tells it, once."""
+import ctypes
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+V = 5000
+
+
+@pytest.fixture(scope="module")
+def gv():
+    import geode_amd
+
+    geode_amd.init(0)
+    return geode_amd
+
+
+class BadRules:
+    """queues a gv_process_logits call one of whose rows names a mask that is not there"""
+
+    def __init__(self, gv):
+        self.gv = gv
+        self.bufs = [gv.DeviceBuffer.from_array(a) for a in (
+            np.zeros((2, V), np.float32), np.full((1, (V + 31) // 32), 0xFFFFFFFF, np.uint32), np.array([0, 1], np.int32))]
+        self.out = gv.DeviceBuffer(2 * V * 4)
+        x, masks, of = self.bufs
+        self.rules = gv.GvLogitsRules(masks=masks.ptr, n_masks=1, ld_mask=(V + 31) // 32, mask_of=of.ptr)
+        gv.check(gv.lib.gv_synchronize(), "gv_synchronize")
+
+    def queue(self):
+        self.gv.check(self.gv.lib.gv_process_logits(ctypes.byref(self.rules), self.bufs[0].ptr, self.gv.F32, V, 2, V,
+                                                    self.out.ptr, V), "gv_process_logits")
+
+
+def _waiting_calls(gv):
+    """(name, a call that waits for results of device memory that is in order)"""
+    r = np.random.default_rng(80)
+    rows = gv.DeviceBuffer.from_array((r.standard_normal((9, V)) * 3).astype(np.float32))
+    batch, out, kept = np.array([7, 8, 9, 10], np.int32), np.zeros(64, np.int32), ctypes.c_int(0)
+    u, uf, seen, stop = np.full(9, 0.5), np.full(9, 0.5, np.float32), np.array([3, 4], np.int32), np.arange(40, dtype=np.int32)
+    host = np.zeros(4, np.float32)
+    p = lambda a: a.ctypes.data   # noqa: E731
+    keep = (rows, batch, out, kept, u, uf, seen, stop, host)
+
+    def match(T, top_k, penalty=0.0, n_stop=0):
+        return lambda: gv.lib.gv_accept_match_ex(rows.ptr, V, V, p(batch), 4, T, 0.9, top_k, 0, p(u), p(seen), 2, penalty,
+                                                 p(stop), n_stop, p(out), ctypes.byref(kept))
+
+    def textbook(T, top_p, greedy):
+        return lambda: gv.lib.gv_accept_textbook(rows.ptr, rows.ptr + 5 * V * 4, V, V, 4, T, top_p, greedy, p(uf), p(uf), 0.5,
+                                                 p(out))
+
+    calls = {
+        "memcpy_d2h": lambda: gv.lib.gv_memcpy_d2h(p(host), rows.ptr, 16),
+        "sample greedy": lambda: gv.lib.gv_sample_rows(rows.ptr, V, 4, V, 0.0, 1.0, 0, 0, p(u), p(out)),
+        "sample": lambda: gv.lib.gv_sample_rows(rows.ptr, V, 4, V, 0.8, 0.9, 0, 0, p(u), p(out)),
+        "match greedy": match(0.0, 0), "match candidates": match(0.8, 50), "match walks": match(0.8, 0),
+        "match penalty": match(0.8, 50, 0.5), "match many stops": match(0.0, 0, 0.0, 40),
+        "textbook greedy": textbook(0.8, 0.9, 1), "textbook candidates": textbook(0.8, 0.9, 0), "textbook walks": textbook(0.8, 1.0, 0),
+    }
+    return calls, keep
+
+
+CALLS = ["memcpy_d2h", "sample greedy", "sample", "match greedy", "match candidates", "match walks", "match penalty",
+         "match many stops", "textbook greedy", "textbook candidates", "textbook walks"]
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_calls_that_hand_out_results_tell_a_fault(gv, name):
+    """a row made of rules that are not there is not turned into tokens or copied out with success; the call after it is
+    as without the fault"""
+    bad = BadRules(gv)
+    calls, keep = _waiting_calls(gv)
+    assert calls[name]() >= 0
+    bad.queue()
+    assert calls[name]() == -1
+    assert "range, bias range or mask" in gv.lib.gv_last_error().decode()
+    assert calls[name]() >= 0
+    gv.check(gv.lib.gv_synchronize(), "gv_synchronize")   # (told once)
+    bad.queue()
+    assert gv.lib.gv_synchronize() == -1
+    assert calls[name]() >= 0
+    del keep
