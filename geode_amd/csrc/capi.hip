@@ -161,9 +161,10 @@ int gv_memcpy_h2d(void *dst, const void *src, size_t bytes) {
 
 int gv_memcpy_d2h(void *dst, const void *src, size_t bytes) {
     if (ensure_init() != 0) return -1;
+    const FaultWait faults;
     GV_CHECK_HIP(hipMemcpyAsync(dst, src, bytes, hipMemcpyDeviceToHost, stream()));
     GV_CHECK_HIP(hipStreamSynchronize(stream()));
-    return take_queued_faults();
+    return faults.told();
 }
 
 int gv_memcpy_d2d(void *dst, const void *src, size_t bytes) {
@@ -182,8 +183,9 @@ int gv_memset(void *dst, int value, size_t bytes) {
 
 int gv_synchronize(void) {
     if (ensure_init() != 0) return -1;
+    const FaultWait faults;
     GV_CHECK_HIP(hipStreamSynchronize(stream()));
-    return take_queued_faults();
+    return faults.told();
 }
 
 int gv_event_record(void) {

@@ -1,9 +1,12 @@
 // paged.hip - the paged cache of several conversations: new rows' keys and values appended to it (gv_paged_append),
 // and what the paged calls share on the host.
 #include <algorithm>
+#include <atomic>
+#include <cstring>
 #include <mutex>
 #include <string>
 #include <type_traits>
+#include <vector>
 
 #include "paged.hpp"
 
@@ -19,38 +22,100 @@ const char *kFaultText[kFaultCount] = {
     "a token range, bias range or mask outside its array",
 };
 
-int *g_fault_host = nullptr, *g_fault_dev = nullptr;
+constexpr int kFaultLine = 16;    // words a host thread's take: a line of 64 bytes
+constexpr int kFaultLines = 64;   // lines allocated at a time (kept until the process ends)
 
-}  // namespace
+struct FaultLine {
+    volatile int *host = nullptr;
+    int *dev = nullptr;
+    uint64_t ended = 0;   // how many threads had ended when its own had, itself among them
+};
+struct FaultLines {
+    std::mutex use;
+    std::vector<FaultLine> idle, ended;   // of no thread; of threads that have ended with calls that may still run
+    std::atomic<uint64_t> ends{0};
+    std::atomic<int> n_ended{0};
+};
+FaultLines &fault_lines() {
+    static FaultLines *lines = new FaultLines;   // (never destroyed: a thread may end after main has)
+    return *lines;
+}
 
-int *queued_faults() {
-    static std::mutex once;   // (calls of several host threads)
-    const std::lock_guard<std::mutex> lock(once);
-    if (g_fault_dev) return g_fault_dev;
+// the calling thread's line, from its first queued call to its end
+struct ThreadLine {
+    FaultLine line;
+    ~ThreadLine() {
+        if (!line.dev) return;
+        FaultLines &all = fault_lines();
+        const std::lock_guard<std::mutex> lock(all.use);
+        line.ended = all.ends.fetch_add(1) + 1;
+        all.ended.push_back(line);
+        all.n_ended.fetch_add(1);
+    }
+};
+thread_local ThreadLine t_line;
+
+int more_lines(FaultLines &all) {
+    constexpr size_t bytes = size_t{kFaultLines} * kFaultLine * sizeof(int);
     void *h = nullptr, *d = nullptr;
-    // (portable: any of the process's GPUs may write it; kept until the process ends)
-    if (hipHostMalloc(&h, 64, hipHostMallocMapped | hipHostMallocPortable) != hipSuccess ||
+    // (portable: any of the process's GPUs may write it)
+    if (hipHostMalloc(&h, bytes, hipHostMallocMapped | hipHostMallocPortable) != hipSuccess ||
         hipHostGetDevicePointer(&d, h, 0) != hipSuccess) {
         (void)hipGetLastError();
         if (h) (void)hipHostFree(h);
         set_error("no pinned memory for the queued calls' faults");
-        return nullptr;
+        return -1;
     }
-    for (int i = 0; i < kFaultCount; ++i) static_cast<int *>(h)[i] = 0;
-    g_fault_host = static_cast<int *>(h);
-    g_fault_dev = static_cast<int *>(d);
-    return g_fault_dev;
+    memset(h, 0, bytes);
+    for (int i = kFaultLines - 1; i >= 0; --i) {
+        FaultLine l;
+        l.host = static_cast<int *>(h) + i * kFaultLine, l.dev = static_cast<int *>(d) + i * kFaultLine;
+        all.idle.push_back(l);
+    }
+    return 0;
 }
 
-int take_queued_faults() {
-    if (!g_fault_host) return 0;
-    std::string msg;
-    for (int i = 0; i < kFaultCount; ++i) {
-        volatile int *w = g_fault_host + i;
-        if (!*w) continue;
-        *w = 0;
-        msg += (msg.empty() ? "a queued call met: " : "; ") + std::string(kFaultText[i]);
+unsigned taken(const FaultLine &l) {   // the kinds met (a bit each), the words cleared
+    unsigned kinds = 0;
+    for (int i = 0; i < kFaultCount; ++i)
+        if (l.host[i]) kinds |= 1u << i, l.host[i] = 0;
+    return kinds;
+}
+
+}  // namespace
+
+int *queued_faults() {
+    if (t_line.line.dev) return t_line.line.dev;
+    FaultLines &all = fault_lines();
+    const std::lock_guard<std::mutex> lock(all.use);
+    if (all.idle.empty() && more_lines(all) != 0) return nullptr;
+    t_line.line = all.idle.back();
+    all.idle.pop_back();
+    return t_line.line.dev;
+}
+
+FaultWait::FaultWait() : ends(fault_lines().ends.load()) {}
+
+int FaultWait::told() const {
+    unsigned kinds = t_line.line.dev ? taken(t_line.line) : 0u;
+    FaultLines &all = fault_lines();
+    if (all.n_ended.load() > 0) {
+        const std::lock_guard<std::mutex> lock(all.use);
+        for (size_t i = 0; i < all.ended.size();) {
+            if (all.ended[i].ended > ends) {   // (it ended after this wait had begun: its calls may not be done)
+                ++i;
+                continue;
+            }
+            kinds |= taken(all.ended[i]);
+            all.idle.push_back(all.ended[i]);
+            all.ended[i] = all.ended.back();
+            all.ended.pop_back();
+            all.n_ended.fetch_sub(1);
+        }
     }
+    std::string msg;
+    for (int i = 0; i < kFaultCount; ++i)
+        if (kinds >> i & 1) msg += (msg.empty() ? "a queued call met: " : "; ") + std::string(kFaultText[i]);
     GV_REQUIRE(msg.empty(), msg);
     return 0;
 }

@@ -14,12 +14,17 @@
 namespace gv {
 
 // ---------------------------------------------------------------- faults met in device memory
-// A kernel that meets one sets its word in pinned host memory (every writer writes 1, past the caches: a volatile store); the
-// calls that wait and hand out results (gv_synchronize, gv_memcpy_d2h, the sampling and acceptance calls) read the words
-// behind their wait, clear them and fail.
+// A kernel that meets one sets its word in pinned host memory (every writer writes 1, past the caches: a volatile store). The
+// words are the host thread's whose call it is. The calls that wait and hand out results (gv_synchronize, gv_memcpy_d2h, the
+// sampling and acceptance calls) read the calling thread's behind their wait, and those of threads that ended before it,
+// clear them and fail.
 enum QueuedFault { kFaultRows = 0, kFaultPage = 1, kFaultPosition = 2, kFaultRange = 3, kFaultCount = 4 };
-int *queued_faults();        // the words as the device addresses them (null: no memory, the error set)
-int take_queued_faults();    // 0, or -1 and a message, the words cleared (behind a wait for the stream)
+int *queued_faults();   // the calling thread's words as the device addresses them (null: no memory, the error set)
+struct FaultWait {      // made before the wait for the library's stream
+    uint64_t ends;      // threads that had ended by then
+    FaultWait();
+    int told() const;   // behind the wait: 0, or -1 and a message, the words cleared
+};
 __device__ inline void queue_fault(int *words, int kind) {
     *reinterpret_cast<volatile int *>(words + kind) = 1;
 }

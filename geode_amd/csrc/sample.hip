@@ -1957,6 +1957,7 @@ int gv_sample_rows(const float *logits, int64_t ld, int rows, int V, float tempe
                    int cap, const double *u, int32_t *out) {
     GV_REQUIRE(V <= kMaxVocab, "gv_sample_rows: a vocabulary of at most 262,144 tokens");
     if (ensure_init() != 0) return -1;
+    const FaultWait faults;
     GV_REQUIRE(logits && out && rows >= 1 && rows <= kSampleRows && V >= 1 && ld >= V, "gv_sample_rows: bad arguments");
     GV_REQUIRE(temperature <= 0.0f || u, "gv_sample_rows: uniforms needed when temperature > 0");
     void *base = ws_mem().get(ws_bytes(rows, 0));
@@ -1972,7 +1973,7 @@ int gv_sample_rows(const float *logits, int64_t ld, int rows, int V, float tempe
     if (nuclei(rs, rows, temperature, top_p, top_k, cap, c.ws, st) != 0) return -1;
     GV_CHECK_HIP(hipMemcpyAsync(pin, c.ws.picks, 4 * static_cast<size_t>(rows), hipMemcpyDeviceToHost, st));
     GV_CHECK_HIP(hipStreamSynchronize(st));
-    if (take_queued_faults() != 0) return -1;
+    if (faults.told() != 0) return -1;
     std::copy(reinterpret_cast<int32_t *>(pin), reinterpret_cast<int32_t *>(pin) + rows, out);
     return 0;
 }
@@ -1989,6 +1990,7 @@ int gv_accept_match_ex(float *logits, int64_t ld, int V, const int32_t *batch, i
                        const int32_t *stop, int n_stop, int32_t *out, int *kept) {
     GV_REQUIRE(V <= kMaxVocab, "gv_accept_match: a vocabulary of at most 262,144 tokens");
     if (ensure_init() != 0) return -1;
+    const FaultWait faults;
     GV_REQUIRE(logits && batch && out && n >= 1 && n <= 32 && V >= 1 && ld >= V, "gv_accept_match: bad arguments");
     GV_REQUIRE(temperature <= 0.0f || u, "gv_accept_match: uniforms needed when temperature > 0");
     GV_REQUIRE(n_seen >= 0 && (n_seen == 0 || seen) && n_seen <= V, "gv_accept_match: seen tokens");
@@ -2059,7 +2061,7 @@ int gv_accept_match_ex(float *logits, int64_t ld, int V, const int32_t *batch, i
                                done, seq);
         }
         GV_CHECK_HIP(hipGetLastError());
-        if (wait_posted(done, seq, st) != 0 || take_queued_faults() != 0) return -1;
+        if (wait_posted(done, seq, st) != 0 || faults.told() != 0) return -1;
         const int emitted = hint[32];
         if (emitted > 0) {
             for (int i = 0; i < emitted; ++i) out[i] = hint[i];
@@ -2087,7 +2089,7 @@ int gv_accept_match_ex(float *logits, int64_t ld, int V, const int32_t *batch, i
         GV_CHECK_HIP(hipGetLastError());
         GV_CHECK_HIP(hipMemcpyAsync(hint, dout, 36 * 4, hipMemcpyDeviceToHost, st));
         GV_CHECK_HIP(hipStreamSynchronize(st));
-        if (take_queued_faults() != 0) return -1;
+        if (faults.told() != 0) return -1;
         const int emitted = hint[32];
         if (emitted > 0) {
             for (int i = 0; i < emitted; ++i) out[i] = hint[i];
@@ -2103,7 +2105,7 @@ int gv_accept_match_ex(float *logits, int64_t ld, int V, const int32_t *batch, i
     GV_CHECK_HIP(hipGetLastError());
     GV_CHECK_HIP(hipMemcpyAsync(hint, dout, 36 * 4, hipMemcpyDeviceToHost, st));
     GV_CHECK_HIP(hipStreamSynchronize(st));
-    if (take_queued_faults() != 0) return -1;
+    if (faults.told() != 0) return -1;
     const int emitted = hint[32];
     for (int i = 0; i < emitted; ++i) out[i] = hint[i];
     if (kept) *kept = hint[33];
@@ -2114,6 +2116,7 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
                        float top_p, int greedy, const float *u_draft, const float *u_acc, float u_res, int32_t *out) {
     GV_REQUIRE(V <= kMaxVocab, "gv_accept_textbook: a vocabulary of at most 262,144 tokens");
     if (ensure_init() != 0) return -1;
+    const FaultWait faults;
     GV_REQUIRE(target && draft && out && k >= 1 && k <= 31 && V >= 1 && ld >= V, "gv_accept_textbook: bad arguments");
     GV_REQUIRE(greedy || (u_draft && u_acc && temperature > 0.0f), "gv_accept_textbook: uniforms and T > 0 needed");
     const int R = 2 * k + 1;
@@ -2148,7 +2151,7 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
         hipLaunchKernelGGL(greedy_finish, dim3(1), dim3(kSortThreads), 0, st, c.ws, rs.S, k, hout, hout + 32, done,
                            seq);
         GV_CHECK_HIP(hipGetLastError());
-        if (wait_posted(done, seq, st) != 0 || take_queued_faults() != 0) return -1;
+        if (wait_posted(done, seq, st) != 0 || faults.told() != 0) return -1;
         const int emitted = hout[32];
         for (int i = 0; i < emitted; ++i) out[i] = hout[i];
         return emitted;
@@ -2174,7 +2177,7 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
         hipLaunchKernelGGL(fast_textbook, dim3(1), dim3(kSortThreads), lds_t, st, rs, c.ws, k, temperature, fu, hout,
                            hout + 32, done, seq);
         GV_CHECK_HIP(hipGetLastError());
-        if (wait_posted(done, seq, st) != 0 || take_queued_faults() != 0) return -1;
+        if (wait_posted(done, seq, st) != 0 || faults.told() != 0) return -1;
         const int emitted = hout[32];
         if (emitted > 0) {
             for (int i = 0; i < emitted; ++i) out[i] = hout[i];
@@ -2191,7 +2194,7 @@ int gv_accept_textbook(const float *target, const float *draft, int64_t ld, int 
     GV_CHECK_HIP(hipGetLastError());
     GV_CHECK_HIP(hipMemcpyAsync(hout, dout, 33 * 4, hipMemcpyDeviceToHost, st));
     GV_CHECK_HIP(hipStreamSynchronize(st));
-    if (take_queued_faults() != 0) return -1;
+    if (faults.told() != 0) return -1;
     const int emitted = hout[32];
     for (int i = 0; i < emitted; ++i) out[i] = hout[i];
     return emitted;

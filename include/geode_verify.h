@@ -37,8 +37,9 @@ int gv_memcpy_d2h(void *dst, const void *src, size_t bytes); /* waits; fails as 
 int gv_memcpy_d2d(void *dst, const void *src, size_t bytes);
 int gv_memset(void *dst, int value, size_t bytes);
 /* Waits for the library's stream. Fails when a queued call met a fault in device memory (the paged calls and
- * gv_process_logits below) that no call has told yet: the first that waits and hands out results does, once - this one,
- * gv_memcpy_d2h, gv_sample_rows or a gv_accept call. */
+ * gv_process_logits below) that was not told yet: the first call that waits and hands out results does, once - this one,
+ * gv_memcpy_d2h, gv_sample_rows or a gv_accept call - of the host thread whose call it was (of a thread that has ended
+ * since: of any). A thread that leaves the reading of its calls' results to another one waits itself first. */
 int gv_synchronize(void);
 /* milliseconds between two points of the library's stream: gv_event_record returns an id */
 int gv_event_record(void);
@@ -397,7 +398,8 @@ int gv_sampler_paths(int64_t *candidate, int64_t *walks);
  * device: a sequence whose row starts or length do not fit, a page outside the pool, a rotary position outside the
  * tables, a token range or mask outside its array. Nothing outside the arrays is read or written for it, what it
  * gives is unspecified, the other sequences and rows are unaffected, and the next call that waits and hands out results
- * (gv_synchronize, gv_memcpy_d2h, gv_sample_rows, the gv_accept calls, which then give nothing) fails with a message. */
+ * of the same host thread (gv_synchronize, gv_memcpy_d2h, gv_sample_rows, the gv_accept calls, which then give nothing)
+ * fails with a message. */
 enum { GV_F32 = 0, GV_F16 = 1, GV_BF16 = 2, GV_I8 = 3 }; /* element types */
 
 /* One layer's paged cache: n_pages pages of page_size positions, keys and values apart. The element (page, head,

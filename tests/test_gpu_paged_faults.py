@@ -1,5 +1,9 @@
-"""What a fault met in device memory reaches: every call that waits and hands out results tells it, once."""
+"""What a fault met in device memory reaches: every call that waits and hands out results tells it, once, to the host thread
+whose call it was."""
 import ctypes
+import threading
+import time
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -83,3 +87,50 @@ def test_calls_that_hand_out_results_tell_a_fault(gv, name):
     assert gv.lib.gv_synchronize() == -1
     assert calls[name]() >= 0
     del keep
+
+
+def test_a_fault_is_told_to_the_thread_whose_call_it_was(gv):
+    """two host threads on the one stream: the thread whose calls are in order waits and gets its results, before and after
+    the other learns of its own fault"""
+    a, b = BadRules(gv), BadRules(gv)
+    b.bufs[2].upload(np.array([0, -1], np.int32))   # (in order)
+    sync = gv.lib.gv_synchronize
+    with ThreadPoolExecutor(1) as one, ThreadPoolExecutor(1) as two:
+        do = lambda t, f: t.submit(f).result()   # noqa: E731
+        for _ in range(3):
+            do(one, a.queue)
+            do(two, b.queue)
+            assert do(two, sync) == 0
+            assert np.array_equal(do(two, lambda: b.out.download(np.float32, (2, V))), np.zeros((2, V), np.float32))
+            assert do(one, sync) == -1
+            assert do(one, sync) == 0 and do(two, sync) == 0 and sync() == 0
+
+
+def test_the_fault_of_a_thread_that_has_ended(gv):
+    """a thread that queued a call and ended without a wait: the next thread that waits is told, once; and many threads one
+    after the other each learn of their own faults alone"""
+    bad = BadRules(gv)
+    t = threading.Thread(target=bad.queue)
+    t.start()
+    t.join()
+    told = []
+    for _ in range(200):   # (the thread's own end comes a little after its join)
+        told.append(gv.lib.gv_synchronize())
+        if told[-1] != 0:
+            break
+        time.sleep(0.01)
+    assert told[-1] == -1 and gv.lib.gv_synchronize() == 0
+    good = BadRules(gv)
+    good.bufs[2].upload(np.array([0, -1], np.int32))
+    said = []
+
+    def work(i):
+        (bad if i % 3 == 0 else good).queue()
+        said.append((gv.lib.gv_synchronize(), gv.lib.gv_synchronize()))
+
+    for i in range(150):
+        t = threading.Thread(target=work, args=(i,))
+        t.start()
+        t.join()
+    assert said == [(-1 if i % 3 == 0 else 0, 0) for i in range(150)]
+    assert gv.lib.gv_synchronize() == 0
