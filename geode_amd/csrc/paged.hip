@@ -200,9 +200,11 @@ __device__ inline double group_sum(double v, int lg) {
     for (int o = lg / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-__device__ inline float group_max(float v, int lg) {
-    for (int o = lg / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+// the largest size of the group's values: of their bits without the sign, which order as the sizes do, a NaN above infinity
+__device__ inline uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ inline float group_size(uint32_t v, int lg) {
+    for (int o = lg / 2; o > 0; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, 64)));
+    return __uint_as_float(v);
 }
 
 template <int TIN>
@@ -349,9 +351,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
         for (int d = 0; d < D; ++d) {
             const float4 y = x[d];
             const bool live = h + d * hw < n;
-            if constexpr (TKV == GV_I8) {   // the row's largest value at 127 steps (quant_kv_row, engine/src/model.cpp:3766-3774)
-                const float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
-                const float amax = group_max(i0 < hd ? m : 0.0f, a.lg);
+            if constexpr (TKV == GV_I8) {
+                // the row's largest value at 127 steps (quant_kv_row, engine/src/model.cpp:3766-3774), but a NaN, which that passes
+                // over, is the largest: the scale is then no number, and the row not one that looks in order
+                const uint32_t m = max(max(size_bits(y.x), size_bits(y.y)), max(size_bits(y.z), size_bits(y.w)));
+                const float amax = group_size(i0 < hd ? m : 0u, a.lg);
                 const float inv = amax > 0.0f ? __fdiv_rn(127.0f, amax) : 0.0f;
                 const auto q8 = [inv](float v) {
                     return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(__fmul_rn(v, inv)), -127.0f), 127.0f))) & 0xFFu;

@@ -435,7 +435,8 @@ typedef struct gv_paged_batch {
 
 /* New rows to the cache: queries and keys RMSNorm'ed (weight 1 + w, the sum of squares in 64 bits) where a weight is
  * given, their first rope_dim values rotated, keys and values rounded once to the cache's type, the queries written
- * to q_out. The model's own arithmetic, value for value (engine/src/model.cpp:3690-3797). */
+ * to q_out. The model's own arithmetic, value for value (engine/src/model.cpp:3690-3797), but for a NaN in a key or value
+ * of an int8 cache: the scale becomes NaN (the model's passes over it; of a row with an infinity both are infinite). */
 typedef struct gv_append_rows {
     int32_t type;             /* GV_F32, GV_F16 or GV_BF16: q, k and v */
     int32_t n_heads;          /* query heads, 0: no queries */
@@ -460,8 +461,9 @@ int gv_paged_append(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv
  * out = sum softmax(scale q . k) v over the positions before the sequence's first new row and, of its new rows, those
  * the row sees: itself and the rows before it, or with `visible` the rows j whose bit j is set. A row that sees
  * nothing gives zeros and lse -inf. What a row does not see does not reach it, NaNs and infinities included; a NaN key that
- * it sees makes the head's result NaN, a NaN or infinite value that dim's result not finite, and infinite keys, NaN or
- * infinite scales of an int8 cache leave the head's result unspecified. Query head h reads KV head h / (n_heads / n_kv_heads). Scores, softmax and sums in fp32, the weights with at
+ * it sees (or NaN scale of an int8 cache) makes the head's result NaN, a NaN or infinite value that dim's result not
+ * finite, and infinite keys or scales leave the head's result unspecified. Query head h reads KV head
+ * h / (n_heads / n_kv_heads). Scores, softmax and sums in fp32, the weights with at
  * least 16 bits (times an int8 cache's value scales, which may be of any size: to 2^-37 of the largest such product). Equal calls give equal bits. */
 typedef struct gv_attention_rows {
     int32_t type;            /* q and out: the cache's type or GV_F32 (GV_I8: GV_F32, GV_F16 or GV_BF16) */

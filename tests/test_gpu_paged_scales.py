@@ -108,3 +108,37 @@ def test_scores_and_scales_of_any_kind(gv, nh, nkv, hd, rows, kind, rise):
         scales.append(e)
     vs = _spanned(f, 75, scores, scales, 8.0)
     _check(gv, f, kind, nh, 8.0, vs)
+
+
+@pytest.mark.parametrize("nh,hd,rows", [(4, 64, 3), (4, 256, 3), (16, 64, 5), (16, 128, 5), (16, 256, 5), (6, 192, 5)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_a_row_that_is_not_finite_is_not_made_finite(gv, nh, hd, rows, which, value):
+    """a NaN or an infinity in a new row's key or value shows in what the cache then holds of that (position, KV head), and a
+    NaN in the results of the rows that see it; other positions, KV heads and rows are as without it"""
+    nkv = 2
+    r = np.random.default_rng(76)
+    q, k, v = (round_to(r.standard_normal((rows, h, hd)), "f32") for h in (nh, nkv, nkv))
+    got = {}
+    for bad in (False, True):
+        f = Filled(77, "i8", [rows], [400], 32, nkv, hd)
+        x = {"k": k.copy(), "v": v.copy()}
+        if bad:
+            x[which][1, 1, hd // 2 + 1] = value
+        gv.paged_append(f.cache, f.batch, None, x["k"], x["v"])
+        got[bad] = (f.cache.read("k"), f.cache.read("v"), *gv.paged_attention(f.cache, f.batch, q))
+    p, s = f.place(0, 400 - rows + 1)
+    n = "kv".index(which)
+    assert not np.isfinite(got[True][n][p, 1, s]).any()
+    for i in (0, 1):
+        a, b = got[False][i].copy(), got[True][i].copy()
+        if i == n:
+            a[p, 1, s] = b[p, 1, s] = 0
+        assert np.array_equal(a, b, equal_nan=True)
+    half = nh // 2
+    for i in (2, 3):
+        assert np.array_equal(got[True][i][0], got[False][i][0])
+        assert np.array_equal(got[True][i][:, :half], got[False][i][:, :half])
+    if np.isnan(value):
+        assert np.isnan(got[True][2][1:, half:]).all()
+        assert np.isfinite(got[False][2]).all()
