@@ -17,8 +17,9 @@
 //
 // Rounding: queries and weights go to the matrix cores as PARTS 16-bit parts (fp16: 11 bits each, bf16: 8), keys and
 // values exactly (int8: as fp16 (code) / 512); products are summed in fp32. A query exact in the cache's type is one
-// part; the weights are two parts for 16-bit results (an error of 2^-16 at most, far below the result's own rounding)
-// and 22 or 24 bits for fp32 ones. fp16 parts are taken of values scaled by powers of two (queries by their row's
+// part, an fp32 one two of fp16 (truncated: 2^-21 at most, down to 2^-35 of its row's largest) or three of bf16 (exact); the
+// weights are two parts (bf16: off by 2^-16 at most, for results of 8 bits; fp16: truncated, by 2^-21) or, for fp32 results
+// over bf16, three (exact). fp16 parts are taken of values scaled by powers of two (queries by their row's
 // largest value, weights by 2^14, an int8 cache's weights x value scales by their largest's: weight_factor), so that neither
 // overflows nor, where it counts, falls below fp16's range.
 // The weights' exponential takes the difference to the maximum: exp2((s - m) log2 e), accurate whatever the scores' size.
@@ -101,7 +102,7 @@ __device__ inline float rows_sum(float v) {
 }
 
 // N parts of K floats in the operand's type, two to a word: each part the leading bits of what the parts before left
-// (truncated, so that the rest is exact)
+// (truncated, so that the rest is exact; the last of bf16 parts rounded to nearest, the same one instruction)
 template <bool BF, int N, int K, typename Part>
 __device__ inline void split_parts(const float (&x)[K], Part &&put) {
     float r[K];
@@ -112,9 +113,11 @@ __device__ inline void split_parts(const float (&x)[K], Part &&put) {
 #pragma unroll
         for (int j = 0; j < K; j += 2) {
             if constexpr (BF) {
-                const uint32_t a = __builtin_bit_cast(uint32_t, r[j]), b = __builtin_bit_cast(uint32_t, r[j + 1]);
-                put(p, j / 2, perm(b, a, 0x07060302u));
-                if (p + 1 < N) {
+                if (p + 1 == N) {
+                    put(p, j / 2, pack_bf16(r[j], r[j + 1]));
+                } else {
+                    const uint32_t a = __builtin_bit_cast(uint32_t, r[j]), b = __builtin_bit_cast(uint32_t, r[j + 1]);
+                    put(p, j / 2, perm(b, a, 0x07060302u));
                     r[j] -= __builtin_bit_cast(float, a & 0xFFFF0000u);
                     r[j + 1] -= __builtin_bit_cast(float, b & 0xFFFF0000u);
                 }
