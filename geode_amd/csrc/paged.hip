@@ -224,10 +224,8 @@ __device__ inline float4 raw_floats(typename Raw4<TIN>::type r) {
 
 // D: heads a lane group takes in a round (their control flow once)
 template <int TIN, int TKV, int D>
-__global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
-    touch_args(a);
-    const int t = blockIdx.x, hd = a.kv.hd, nkv = a.kv.nkv, lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+__device__ inline void append_row(const AppendArgs &a, int t, int wave) {
+    const int hd = a.kv.hd, nkv = a.kv.nkv, lane = threadIdx.x & 63;
     const int l = lane & (a.lg - 1), i0 = 4 * l, hw = 64 / a.lg, in_round = lane / a.lg;
     const int ic = min(i0, hd - 4);
     constexpr int es = TIN == GV_F32 ? 4 : 2;
@@ -249,7 +247,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
     if (a.k_norm) wk = *reinterpret_cast<const float4 *>(a.k_norm + ic);
 
     Seq s;
-    const int i = seq_of_row(a.b, t, s);
+    bool misfit;
+    const int i = seq_of_row(a.b, t, s, misfit);
+    if (misfit && lane == 0) queue_fault(a.faults, kFaultRows);   // (whichever rows it has, and also none)
     if (i >= a.b.n_seqs) return;   // a row behind the last sequence
     if (t < s.first && i == 0) return;   // a row before the first sequence
     if (!s.fits || t < s.first || t >= s.first + s.rows) {
@@ -368,6 +368,14 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
             }
         }
     } while (more);
+}
+
+template <int TIN, int TKV, int D>
+__global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
+    touch_args(a);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    append_row<TIN, TKV, D>(a, static_cast<int>(blockIdx.x), wave);
+    if (a.b.n_seqs > 64 && blockIdx.y == 0 && wave == 0) check_sequences(a.b, static_cast<int>(blockIdx.x), a.faults);
 }
 
 template <int TIN, int D>

@@ -94,9 +94,8 @@ __device__ inline Seq seq_load(const BatchView &b, int i) { return make_seq(b, b
 
 // The sequence of row t, the first whose rows end behind t (n_seqs: none), and what the batch says of it. A 64-way search
 // by a whole wave, one round of loads up to 64 sequences, two up to 4,096; the last round's lanes hold their sequences'
-// starts and lengths too. Row starts that descend give some sequence of the batch, which its own check (or the row's place
-// in it) refuses.
-__device__ inline int seq_of_row(const BatchView &b, int t, Seq &s) {
+// starts and lengths too (misfit: one of those does not fit). Row starts that descend give some sequence of the batch.
+__device__ inline int seq_of_row(const BatchView &b, int t, Seq &s, bool &misfit) {
     const int lane = threadIdx.x & 63;
     const int *end = b.row_start + 1;
     int lo = 0, hi = b.n_seqs;
@@ -109,10 +108,19 @@ __device__ inline int seq_of_row(const BatchView &b, int t, Seq &s) {
     }
     const int i = lo + lane, ic = min(i, b.n_seqs - 1);
     const int first = b.row_start[ic], last = end[ic], len = b.lens[ic];
+    misfit = __any(!make_seq(b, first, last, len).fits);   // (lanes past the last sequence: the last again)
     const int at = __popcll(__ballot(i < hi && last <= t));   // (64: behind all of them)
     const int src = min(at, 63);
     s = make_seq(b, __builtin_amdgcn_readlane(first, src), __builtin_amdgcn_readlane(last, src), __builtin_amdgcn_readlane(len, src));
     return lo + at < hi ? lo + at : b.n_seqs;
+}
+
+// A wave's share of the check of every sequence, row t's: of more than a row's search looks at
+__device__ inline void check_sequences(const BatchView &b, int t, int *faults) {
+    for (int64_t i0 = int64_t{64} * t; i0 < b.n_seqs; i0 += int64_t{64} * b.n_rows) {
+        const int64_t i = i0 + (threadIdx.x & 63);
+        if (i < b.n_seqs && !seq_load(b, static_cast<int>(i)).fits) queue_fault(faults, kFaultRows);
+    }
 }
 
 // 32-bit floats to the 16-bit types, rounded to nearest even
@@ -130,17 +138,7 @@ __device__ inline float half_hi(uint32_t w) { return static_cast<float>(__builti
 __device__ inline float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
 __device__ inline float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xFFFF0000u); }
 
-// four consecutive values of a type as floats (16 or 8 bytes, aligned), and four floats stored as a type
-template <int TYPE>
-__device__ inline float4 load4(const char *p) {
-    if constexpr (TYPE == GV_F32) {
-        return *reinterpret_cast<const float4 *>(p);
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p);
-        if constexpr (TYPE == GV_F16) return float4{half_lo(w.x), half_hi(w.x), half_lo(w.y), half_hi(w.y)};
-        return float4{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
-    }
-}
+// four floats stored as a type (16 or 8 bytes, aligned)
 template <int TYPE>
 __device__ inline void store4(char *p, float4 x) {
     if constexpr (TYPE == GV_F32) *reinterpret_cast<float4 *>(p) = x;

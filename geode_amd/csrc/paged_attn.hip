@@ -28,7 +28,8 @@ __global__ __launch_bounds__(GROUPS * kJoinLanes) void paged_join_kernel(const J
     const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
     const int grp = tid / kJoinLanes, l16 = tid % kJoinLanes, d = blockIdx.z * kJoinDims + 4 * l16;
     Seq s;
-    if (seq_of_row(a.b, row, s) >= a.b.n_seqs) return;
+    bool misfit;   // (told by the first launch)
+    if (seq_of_row(a.b, row, s, misfit) >= a.b.n_seqs) return;
     if (!s.fits || row < s.first || row >= s.first + s.rows || s.len <= a.chunk) return;
     const int nc = (s.len + a.chunk - 1) / a.chunk;
     const int64_t step = static_cast<int64_t>(a.b.n_rows) * a.nh, at = static_cast<int64_t>(row) * a.nh + head;

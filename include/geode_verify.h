@@ -397,7 +397,8 @@ int gv_sampler_paths(int64_t *candidate, int64_t *walks);
  * What the host passes is checked by the call (nonzero, gv_last_error). What lies in device memory is checked on the
  * device: a sequence whose row starts or length do not fit, a page outside the pool, a rotary position outside the
  * tables, a token range or mask outside its array. Nothing outside the arrays is read or written for it, what it
- * gives is unspecified, the other sequences and rows are unaffected, and the next call that waits and hands out results
+ * gives is unspecified, the other sequences and rows are unaffected (unless row starts descend: then what the whole call
+ * gives is unspecified), and the next call that waits and hands out results
  * of the same host thread (gv_synchronize, gv_memcpy_d2h, gv_sample_rows, the gv_accept calls, which then give nothing)
  * fails with a message. */
 enum { GV_F32 = 0, GV_F16 = 1, GV_BF16 = 2, GV_I8 = 3 }; /* element types */
@@ -421,7 +422,7 @@ typedef struct gv_paged_kv {
 /* The rows of one step: sequence i has rows row_start[i] .. row_start[i + 1] - 1 (row_start[0] >= 0, never descending;
  * rows before the first and from row_start[n_seqs] on belong to none and are left as they are) and lens[i] positions in
  * the cache, its new rows the last of them: its j-th of n rows is position lens[i] - n + j. Position p lies in page
- * pages[i * ld_pages + p / page_size]; entries past the last position are not read. Sequences may share pages that
+ * pages[i * ld_pages + p / page_size]; entries past the last position are not used. Sequences may share pages that
  * no new row goes to. */
 typedef struct gv_paged_batch {
     int32_t n_seqs, n_rows;  /* n_rows: the rows the step's arrays hold, below 2^24 */

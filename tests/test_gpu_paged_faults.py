@@ -134,3 +134,25 @@ def test_the_fault_of_a_thread_that_has_ended(gv):
         t.join()
     assert said == [(-1 if i % 3 == 0 else 0, 0) for i in range(150)]
     assert gv.lib.gv_synchronize() == 0
+
+
+@pytest.mark.parametrize("start", [
+    [2, 1, 4], [0, 3, 2, 4],
+    # (300 sequences, the row starts of two without rows exchanged: no row of the batch lies in either)
+    list(range(100)) + [100] * 150 + [101, 100] + [101 + i for i in range(49)]])
+def test_row_starts_that_descend_are_told_whichever_rows_they_give(gv, start):
+    """also where every row of the batch lies in a sequence that fits"""
+    n, hd, page = len(start) - 1, 16, 16
+    rows = max(start)
+    cache = gv.PagedCache(gv.F16, n, page, 1, hd)
+    good = np.minimum(np.arange(n + 1), rows)
+    batch = gv.PagedBatch(np.diff(good), np.full(n, 16), np.arange(n)[:, None], n_rows=rows, max_rows=16)
+    z = np.zeros((rows, 1, hd))
+    gv.paged_append(cache, batch, z, z, z)
+    gv.paged_attention(cache, batch, z)
+    batch.bufs[0].upload(np.array(start, np.int32))
+    with pytest.raises(gv.GeodeError, match="row starts"):
+        gv.paged_append(cache, batch, z, z, z)
+    with pytest.raises(gv.GeodeError, match="row starts"):
+        gv.paged_attention(cache, batch, z)
+    gv.check(gv.lib.gv_synchronize(), "gv_synchronize")
