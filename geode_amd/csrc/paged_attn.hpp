@@ -158,14 +158,13 @@ __device__ inline uint32_t i8_pair(uint32_t hi, uint32_t lo, uint32_t sel) {
 constexpr float kI8Unit = 512.0f;   // a code's operand x this is the code
 
 // An int8 cache's weights take the value scales with them, times a power of two that brings a column's largest weight x scale
-// to 2^13 .. 2^14 (of all scales, whatever their weight, it would push the weights that count below fp16's range). top: log2 of
-// the largest weight x scale before the weights' division by e^m, m the largest score; the factor is held between 2^-114 and
-// 2^126 (weights x scales below 2^-113 lose bits). Nothing seen yet: top and m are -inf, their difference no number, the
-// factor the largest.
+// to 2^13 .. 2^14 (of all scales, whatever their weight, it would push the weights that count below fp16's range). most: log2 of
+// the largest weight x scale so far, relative to the largest score (differences of scores alone, so that the scores' size costs
+// it nothing); -inf: nothing seen yet. The factor is held between 2^-114 and 2^126 (weights x scales below 2^-113 lose bits).
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMostFactor = 126;
-__device__ inline float weight_factor(float top, float m) {
-    const float e = fminf(fmaxf(floorf(__builtin_fmaf(-m, kLog2e, top)), 13.0f - kMostFactor), 127.0f);
+__device__ inline float weight_factor(float most) {
+    const float e = fminf(fmaxf(floorf(most), 13.0f - kMostFactor), 127.0f);
     return __builtin_amdgcn_ldexpf(1.0f, 13 - static_cast<int>(e));
 }
 // log2 of one power of two over another
@@ -490,12 +489,12 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
     const int qes = a.type == GV_F32 ? 4 : 2;
 
     float sc[CT], m[CT], l[CT];           // a column's score factor, maximum, sum
-    float most[CT], up[CT];               // its weights' factor for the products; int8: log2 of the largest weight x scale e^m
+    float most[CT], up[CT];               // int8: log2 of the largest weight x scale; its weights' factor for the products
     uint32_t bits[CT];                    // which of the sequence's rows it sees
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         sc[ct] = a.scale * qs.undo(ct) * (I8 ? kI8Unit : 1.0f);
-        m[ct] = most[ct] = -INFINITY, l[ct] = 0.0f, up[ct] = I8 ? weight_factor(-INFINITY, -INFINITY) : 16384.0f;
+        m[ct] = most[ct] = -INFINITY, l[ct] = 0.0f, up[ct] = I8 ? weight_factor(-INFINITY) : 16384.0f;
         bits[ct] = seen_rows(a, u, q0 + ct * 16 + i16);
     }
     af4 acc[CT][NT];
@@ -575,7 +574,7 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                     if (seen && !(hole >> j & 1)) see[ct] |= 1u << j;
                 }
             }
-            float top = -INFINITY, wtop = -INFINITY;
+            float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float f = sc[ct];
@@ -586,17 +585,22 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                     if constexpr (I8) vs[j] = see[ct] >> j & 1 ? vs[j] : 0.0f;
                 }
                 top = fmaxf(top, x[j]);
-                if constexpr (I8) wtop = fmaxf(wtop, __builtin_fmaf(x[j], kLog2e, vlog[j]));
             }
-            top = rows_max(top);
-            if constexpr (I8) wtop = rows_max(wtop);
-            const float mn = fmaxf(m[ct], top), wn = I8 ? fmaxf(most[ct], wtop) : -INFINITY;
+            const float mn = fmaxf(m[ct], rows_max(top));
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            float wn = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = (x[j] - base) * kLog2e;
+                if constexpr (I8) wn = fmaxf(wn, x[j] + vlog[j]);
+            }
+            const float down = mn == m[ct] ? 0.0f : (m[ct] - mn) * kLog2e;
+            if constexpr (I8) wn = fmaxf(rows_max(wn), most[ct] + down);
             if (__any(mn > m[ct] || wn > most[ct])) {
-                const float down = mn == -INFINITY ? 0.0f : (m[ct] - mn) * kLog2e;
                 float f = __builtin_amdgcn_exp2f(down);
                 l[ct] *= f;
                 if constexpr (I8) {   // (at most about 2, whatever its two parts are)
-                    const float now = weight_factor(wn, mn);
+                    const float now = weight_factor(wn);
                     f = __builtin_amdgcn_exp2f(down + log2_ratio(now, up[ct]));
                     most[ct] = wn, up[ct] = now;
                 }
@@ -604,11 +608,10 @@ __device__ inline void attn_few_columns(const AttnArgs &a, const AttnUnit &u) {
                 for (int n = 0; n < NT; ++n) acc[ct][n] *= f;
                 m[ct] = mn;
             }
-            const float base = mn == -INFINITY ? 0.0f : mn;
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
+                x[j] = __builtin_amdgcn_exp2f(x[j]);
                 sum += x[j];
                 if constexpr (I8) {   // (weight x scale first: the scale alone may be far above the largest of them)
                     x[j] = x[j] * vs[j] * up[ct];

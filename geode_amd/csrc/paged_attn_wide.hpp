@@ -132,7 +132,7 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         sc[ct] = a.scale * qs.undo(ct) * (I8 ? kI8Unit : 1.0f);
-        m[ct] = most[ct] = -INFINITY, l[ct] = 0.0f, up[ct] = I8 ? weight_factor(-INFINITY, -INFINITY) : 16384.0f;
+        m[ct] = most[ct] = -INFINITY, l[ct] = 0.0f, up[ct] = I8 ? weight_factor(-INFINITY) : 16384.0f;
         bits[ct] = seen_rows(a, u, u.q0 + ct * 16 + i16);
     }
     af4 acc[4][CT];
@@ -191,7 +191,6 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
             af4 x = part[ct][0];
 #pragma unroll
             for (int q = 1; q < QP; ++q) x += part[ct][q];
-            float wtop = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 x[r] *= I8 ? sc[ct] * f[r] : sc[ct];
@@ -200,11 +199,16 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
                     const bool seen = use && pos < p1 && (pos < ctx || (bits[ct] >> ((pos - ctx) & 31) & 1));
                     x[r] = seen ? x[r] : -INFINITY;
                 }
-                if constexpr (I8) wtop = fmaxf(wtop, __builtin_fmaf(x[r], kLog2e, vlog[r]));
             }
             sv[ct] = x;
             const float top = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-            if constexpr (I8) wtop = rows_max(wtop);
+            float wtop = -INFINITY;   // log2 of the largest weight x scale, relative to `top`
+            if constexpr (I8) {
+                const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) wtop = fmaxf(wtop, __builtin_fmaf(x[r] - base, kLog2e, vlog[r]));
+                wtop = rows_max(wtop);
+            }
             if (lane < 16) {
                 lds_max[t & 1][wave][ct * 16 + lane] = top;
                 if constexpr (I8) lds_wmax[t & 1][wave][ct * 16 + lane] = wtop;
@@ -216,18 +220,20 @@ __device__ inline void attn_many_columns(const AttnArgs &a, const AttnUnit &u) {
         const bool tail = p0 + kRound * t + 16 * wave + 16 > ctx || !(at.usable >> (4 * t + wave) & 1);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            float mn = m[ct], wn = most[ct];
+            float mn = m[ct], theirs[kAttnWaves];
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) {
-                mn = fmaxf(mn, lds_max[t & 1][w][ct * 16 + i16]);
-                if constexpr (I8) wn = fmaxf(wn, lds_wmax[t & 1][w][ct * 16 + i16]);
-            }
+            for (int w = 0; w < kAttnWaves; ++w) theirs[w] = lds_max[t & 1][w][ct * 16 + i16], mn = fmaxf(mn, theirs[w]);
+            const float down = mn == m[ct] ? 0.0f : (m[ct] - mn) * kLog2e;
+            float wn = most[ct] + down;
+            if constexpr (I8)
+#pragma unroll
+                for (int w = 0; w < kAttnWaves; ++w)   // (of a wave that saw nothing: -inf, or no number, which is passed over)
+                    wn = fmaxf(wn, __builtin_fmaf(theirs[w] - mn, kLog2e, lds_wmax[t & 1][w][ct * 16 + i16]));
             if (__any(mn > m[ct] || wn > most[ct])) {
-                const float down = mn == -INFINITY ? 0.0f : (m[ct] - mn) * kLog2e;
                 float f = __builtin_amdgcn_exp2f(down);
                 l[ct] *= f;
                 if constexpr (I8) {
-                    const float now = weight_factor(wn, mn);
+                    const float now = weight_factor(wn);
                     f = __builtin_amdgcn_exp2f(down + log2_ratio(now, up[ct]));
                     most[ct] = wn, up[ct] = now;
                 }

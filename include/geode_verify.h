@@ -464,8 +464,9 @@ int gv_paged_append(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv
  * nothing gives zeros and lse -inf. What a row does not see does not reach it, NaNs and infinities included; a NaN key that
  * it sees (or NaN scale of an int8 cache) makes the head's result NaN, a NaN or infinite value that dim's result not
  * finite, and infinite keys or scales leave the head's result unspecified. Query head h reads KV head
- * h / (n_heads / n_kv_heads). Scores, softmax and sums in fp32, the weights with at
- * least 16 bits (times an int8 cache's value scales, which may be of any size: to 2^-37 of the largest such product). Equal calls give equal bits. */
+ * h / (n_heads / n_kv_heads). Scores, softmax and sums in fp32; the products take fp32 queries with at least 21 bits, to 2^-35
+ * of the row and head's largest (over a bf16 cache exactly), and the weights (of an int8 cache: times the value scales, of
+ * any size) with at least 16 bits, to 2^-37 of the largest. Equal calls give equal bits. */
 typedef struct gv_attention_rows {
     int32_t type;            /* q and out: the cache's type or GV_F32 (GV_I8: GV_F32, GV_F16 or GV_BF16) */
     int32_t n_heads;         /* a multiple of n_kv_heads */

@@ -142,3 +142,28 @@ def test_a_row_that_is_not_finite_is_not_made_finite(gv, nh, hd, rows, which, va
     if np.isnan(value):
         assert np.isnan(got[True][2][1:, half:]).all()
         assert np.isfinite(got[False][2]).all()
+
+
+@pytest.mark.parametrize("nh,nkv,hd", SHAPES)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("score", [3e7, 1e9, -1e9, 1e15])
+def test_large_equal_scores(gv, nh, nkv, hd, rows, score):
+    """positions of one and the same key, whatever the score's size: the plain mean of their values, of scales 1 to 2^20"""
+    lens = [90, 700]
+    f = Filled(78, "i8", rows, lens, 32, nkv, hd)
+    r = np.random.default_rng(79)
+    # (_spanned gives keys of at most 0 in dim 0: the query's sign makes the score's)
+    vs = _spanned(f, 80, [np.full(n, -1.0) for n in lens], [r.uniform(0.0, 20.0, n) for n in lens], 1.0)
+    T = f.batch.desc.n_rows
+    q = np.zeros((T, nh, hd))
+    q[..., 0] = -score
+    out, lse = gv.paged_attention(f.cache, f.batch, round_to(q, "f32"), scale=1.0)
+    for i, n in enumerate(lens):
+        for t in range(f.start[i], f.start[i + 1]):
+            seen = n - f.rows[i] + t - f.start[i] + 1
+            for h in range(nh):
+                v = f.sequence("v", i)[h // (nh // nkv), :seen]
+                # every weight is 1: the scales' 22 bits (2^-21), the sums' roundings (fewer than 64 of 2^-24)
+                tol = np.abs(v).mean(0) * 2.0 ** -17 + vs[np.isfinite(vs)].max() * 127 * 2.0 ** -36
+                assert (np.abs(out[t, h] - v.mean(0)) <= tol).all(), (i, t, h)
+    assert np.isfinite(lse).all()
