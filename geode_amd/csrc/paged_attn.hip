@@ -106,7 +106,8 @@ static AttnPlan attn_plan(const gv_paged_kv &kv, const gv_paged_batch &b, int n_
     // The chunk whose workgroups end first, by what a workgroup takes: some rounds' time to begin and end, and its chunk's rounds.
     double best = 0.0;
     if (wide) {
-        // Rounds of 64 positions, seven to begin and end; the lengths of several sequences taken as three fifths of the longest.
+        // Rounds of 64 positions, seven to begin and end; the lengths of several sequences taken as three fifths of the longest
+        // (a guess at their spread).
         // Two workgroups share a CU's units where their LDS and registers leave room (one alone takes 0.82 of the time it takes
         // beside another). Measured, chunks of 256 / 320 / 384 / 512: 32 sequences of up to 4,096 positions and 5 rows (16 heads
         // of 256, fp16) 41 / 36 / 38 / 44 us; one of 32,001 positions and 17 rows (int8) 56 / 61 / 45 / 51; chunks of 128 / 256 /

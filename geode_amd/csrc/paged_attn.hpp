@@ -803,8 +803,9 @@ int launch_attn_one(const AttnArgs &a, unsigned grid, hipStream_t st) {
 // The units by max_len, or COUNTED in as many workgroups as are there at once: where there are more than 32 units a CU. An
 // empty workgroup keeps its place for a microsecond, so that a batch with one long sequence spends its time on them: one
 // of 65,537 positions among thirty short ones (24 heads of 80, bf16; 16,000 units, most of them empty) 45 us by max_len,
-// 24 counted; 64 full sequences of 8,192 (8,192 units) 137 and 139. Each unit scans the lengths, so only up to
-// kCountSeqs sequences.
+// 24 counted; 64 full sequences of 8,192 (8,192 units) 137 and 139. With heads of 256 (fp16), where the counted form has one
+// wave a SIMD and the other two: one of 131,072 among 63 short ones 113 and 86, 32 full ones of 131,072 (16,384 units) 1,593
+// and 1,615. Each unit scans the lengths, so only up to kCountSeqs sequences.
 constexpr int kCountUnits = 32 * 256, kCountSeqs = 256;
 template <int KV, int QP, int PP, int NT, bool EX, int CT>
 int launch_attn_few(const AttnArgs &a, unsigned grid, hipStream_t st) {

@@ -11,9 +11,10 @@
 // The columns' maximum over the round has to be known to all four waves before the weights are made: it goes through LDS
 // too, a round ahead of its use. A round between two barriers: O^T of the round before; the weights of this round; S^T and
 // the maxima of the next - one barrier a round, the weights and maxima in two buffers.
-// Bound by the vector instructions (the softmax of every column, int8 codes made fp16) beside the products: 32 sequences of
-// up to 4,096 positions and 5 rows, 16 heads of 256 on 2, fp16 (108 MB) 35 us; one of 32,001 positions and 17 rows, int8: 44 us,
-// of which a SIMD spends 18 on those and 7.5 on products.
+// 32 sequences of up to 4,096 positions and 5 rows, 16 heads of 256 on 2, fp16 (108 MB) 36 us, in which CT tiles are worked also
+// where a sequence has columns for one; one of 32,001 positions and 17 rows, int8: 45 us, of which a SIMD spends 18.7 on the
+// vector instructions (the softmax of every column, int8 codes made fp16) and 7.5 on products. The rest are waits: keys and
+// values are asked for one round ahead, each round ends in a barrier, and the LDS (74 KB) leaves room for two workgroups a CU.
 #pragma once
 
 #include "paged_attn.hpp"

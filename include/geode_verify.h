@@ -479,8 +479,8 @@ typedef struct gv_attention_rows {
     const uint32_t *visible; /* [n_rows] or NULL: a chain */
 } gv_attention_rows;
 /* Scratch of one call (0: none needed, or arguments that the call refuses). Calls may share it: the library's stream runs
- * them one after the other. It holds partial results for max_len positions, whatever the lengths turn out to be; a
- * smaller max_len is cut finer and may need more. */
+ * them one after the other. It holds partial results for max_len positions, whatever the lengths turn out to be: n_rows
+ * n_heads (head_dim + 2) floats for each 128 to 512 of them; a smaller max_len is cut finer and may need more. */
 size_t gv_paged_attention_workspace_bytes(const gv_paged_kv *kv, const gv_paged_batch *batch, int n_heads);
 int gv_paged_attention(const gv_paged_kv *kv, const gv_paged_batch *batch, const gv_attention_rows *rows, void *ws,
                        size_t ws_bytes);
